@@ -55,6 +55,7 @@ extern "C" {
 #define TVR_DEV_TIMEOUT_CONVERT 5  /* 3xTF32 converter gave up waiting for a stage  */
 #define TVR_DEV_TIMEOUT_PEER 6     /* a cross-rank barrier gave up waiting for a rank */
 #define TVR_DEV_CACHE_FULL 7       /* a KV-cache append past the cache's capacity was dropped */
+#define TVR_DEV_BAD_INDEX 8        /* a page id, slot or row index out of range was dropped */
 
 /* GEMM precision modes */
 #define TVR_GEMM_AUTO 0    /* TVARANT_GEMM_MODE env, else 3xTF32               */
@@ -300,6 +301,111 @@ int tvr_attention_decode_append(const float* q, const float* k_new, const float*
 /* *counter += delta on the stream (an int64 in device memory). */
 int tvr_counter_add(int64_t* counter, int64_t delta, void* stream);
 
+/* ---- paged KV cache: many requests of different lengths -----------------
+ * Keys and values live in pages of `page_size` positions; request r's
+ * position j is row j % page_size of page block_table[r][j / page_size].
+ * Nothing here needs a length on the host, so a step captured in a CUDA graph
+ * serves requests as they grow, finish and start.  No reference counterpart:
+ * the reference has no KV cache. */
+
+/* element types of pages */
+#define TVR_PAGE_F32 0
+#define TVR_PAGE_F16 1  /* rounded to nearest even; values past 65504 become infinities */
+#define TVR_PAGE_BF16 2 /* rounded to nearest even */
+
+/* The pages of one layer: k_pages and v_pages hold [num_pages, kv_heads,
+ * page_size, head_dim] elements of page_type, each given by its element
+ * strides over (page, head, position) with a contiguous last dimension. */
+typedef struct tvr_paged_kv {
+  void* k_pages;
+  void* v_pages;
+  int32_t page_type;
+  int32_t reserved; /* 0 */
+  int64_t num_pages;
+  int64_t page_size;
+  int64_t kv_heads;
+  int64_t head_dim;
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+} tvr_paged_kv;
+
+/* The page pool shared by all layers: block_table [requests, max_pages] (row
+ * stride table_stride) of page ids, and a stack free_pages [num_pages] whose
+ * first *free_count entries are the free pages. */
+typedef struct tvr_page_pool {
+  int32_t* block_table;
+  int64_t table_stride;
+  int64_t max_pages;
+  int64_t requests;
+  int32_t* free_pages;
+  int64_t num_pages;
+  int64_t page_size;
+} tvr_page_pool;
+
+/* One step's block tables and slot maps from request lengths, all of it on
+ * the device.  seq_lens[r] positions of request r are in the cache and
+ * new_lens[r] tokens join it; new_lens[r] < 0 ends the request.
+ *   - Ended requests give up their pages: these go on top of the free stack
+ *     in the order of the requests and of their tables; the length becomes 0.
+ *   - Request r needs ceil((seq + new) / page_size) - ceil(seq / page_size)
+ *     pages.  In the order of the requests, pages are taken from the top of
+ *     the stack and appended to the request's table row.  The first request
+ *     that needs more pages than are left is refused, and so is every later
+ *     one that needs a page; so is one that would exceed max_pages or whose
+ *     tokens exceed the token arrays.  A refused request keeps its length and
+ *     its table, and TVR_DEV_CACHE_FULL is set in the device status word.
+ *   - The tokens lie packed in the order of the requests (tokens_per_request
+ *     0: request r's token i at index i + sum of the earlier requests' new
+ *     lengths), or in rows (token i of request r at r * tokens_per_request +
+ *     i).  For each of `tokens` entries: slots = page * page_size + row of
+ *     its page, -1 for a refused request's token and for padding; positions =
+ *     seq + i (0 for padding); rows = the request (-1 for padding).
+ *     positions and rows may be NULL.
+ * seq_lens_out and free_count_out receive the lengths and the stack's count
+ * after the step and may be seq_lens and free_count themselves; with buffers
+ * of their own, the same call again gives the same result.  At most 8192
+ * requests (TVR_ERR_UNSUPPORTED above). */
+int tvr_page_plan(const tvr_page_pool* pool, const int32_t* seq_lens, const int32_t* new_lens,
+                  int32_t* seq_lens_out, const int32_t* free_count, int32_t* free_count_out,
+                  int64_t* slots, int32_t* positions, int32_t* rows, int64_t tokens,
+                  int64_t tokens_per_request, void* stream);
+
+/* Writes rows of new keys and values, k_new and v_new [tokens, kv_heads,
+ * head_dim] fp32 (strides: the element strides of k_new over (token, head),
+ * then those of v_new; last dimension contiguous), rounded to the pages'
+ * type, into their slots.  A negative slot is skipped; one past the pages is
+ * skipped and sets TVR_DEV_BAD_INDEX.  Two tokens of one call must not share
+ * a slot. */
+int tvr_paged_append(const tvr_paged_kv* cache, const float* k_new, const float* v_new,
+                     const int64_t* strides, const int64_t* slots, int64_t tokens, void* stream);
+
+/* Attention of one new token per request over its own pages:
+ *   out[r, h] = softmax_j(scale q[r, h] . k[r, g, j]) v[r, g, j],
+ *   g = h / (heads / kv_heads), j < seq_lens[r],
+ * and lse[r, h] (NULL: not wanted), the natural-log log-sum-exp.  A request
+ * of length 0 (or less) gives a zero row and lse = -inf; a length past the
+ * table counts as max_pages * page_size.  Products and sums are fp32 whatever
+ * the pages' type.  q and out are [requests, heads, head_dim], k_new and
+ * v_new [requests, kv_heads, head_dim], fp32; strides holds the (request,
+ * head) element strides of q, k_new, v_new and out, in that order.
+ * With k_new, v_new and slots (all three or none) the call also appends: for
+ * slots[r] >= 0, position seq_lens[r] - 1 is taken from k_new / v_new (rounded
+ * to the pages' type) and written to slots[r], which has to be that
+ * position's slot: the same as tvr_paged_append and then this call.
+ * A page id or slot out of range is dropped (the position does not count)
+ * and sets TVR_DEV_BAD_INDEX.  head_dim is at most 256 (TVR_ERR_UNSUPPORTED
+ * above).  `workspace` is device memory of tvr_paged_attention_workspace
+ * bytes, zeroed before its first use, that no two calls use at the same time;
+ * each call leaves it ready for the next. */
+int tvr_paged_attention(const tvr_paged_kv* cache, const float* q, const float* k_new,
+                        const float* v_new, const int64_t* slots, const int32_t* block_table,
+                        int64_t table_stride, int64_t max_pages, const int32_t* seq_lens,
+                        float* out, float* lse, int64_t requests, int64_t heads,
+                        const int64_t* strides, float scale, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int tvr_paged_attention_workspace(int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                  int64_t* bytes);
+
 /* Batched C[i] = A[i] * op(B[i]) for i < batch, each as tvr_gemm_bias_act
  * with alpha 1, beta 0, no activation; matrices are dense row-major with the
  * given element strides between batch entries (stride_b may be 0 to
@@ -396,6 +502,57 @@ int tvr_where(const void* cond, const void* a, const void* b, void* out, int ele
  * No reference kernel: the reference runs argmax on the CPU through its
  * boxed fallback (csrc/aten/Ops.cpp:499-501). */
 int tvr_argmax_rows(const float* x, int64_t* out, int64_t rows, int64_t n, void* stream);
+
+/* What tvr_adjust_logits applies; an absent part has a NULL pointer. */
+typedef struct tvr_logit_rules {
+  /* token histories [rows, tokens_stride], int32 (token_bits 32) or int64
+   * (64): the prompt is entries [0, prompt_lens[r]) (NULL: 0), what was
+   * generated [prompt_lens[r], total_lens[r]).  Ids outside [0, vocab) are
+   * ignored. */
+  const void* tokens;
+  int32_t token_bits;
+  int32_t reserved; /* 0 */
+  int64_t tokens_stride;
+  const int32_t* prompt_lens;
+  const int32_t* total_lens;
+  /* per row (NULL: 1, 0, 0) */
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  /* sparse biases [rows, bias_stride], the first bias_counts[r] of each row
+   * (NULL: all); ids outside [0, vocab) are ignored */
+  const int32_t* bias_ids;
+  const float* bias_values;
+  const int32_t* bias_counts;
+  int64_t bias_stride;
+  /* grammar masks [n_masks, mask_stride] of 32-bit words, bit v % 32 of word
+   * v / 32 set where token v is allowed; row r uses mask mask_rows[r] (NULL:
+   * mask r), none if that is negative */
+  const uint32_t* masks;
+  int64_t mask_stride;
+  int64_t n_masks;
+  const int32_t* mask_rows;
+} tvr_logit_rules;
+
+/* out[r, v] = logits[r, v] adjusted, in this order:
+ *   token v in row r's history:  l = l > 0 ? l / repetition : l * repetition
+ *   c times among the generated: l = l - frequency * c, then - presence if c
+ *   biases of token v:           l = l + value, in the order of the list
+ *   token v not allowed:         l = -inf, whatever the above gave
+ * each operation rounded to fp32.  Rows have strides of their own; out may be
+ * logits (with the same stride).  A mask row index >= n_masks sets
+ * TVR_DEV_BAD_INDEX and masks nothing.  No reference counterpart. */
+int tvr_adjust_logits(const float* logits, int64_t logits_stride, float* out, int64_t out_stride,
+                      int64_t rows, int64_t vocab, const tvr_logit_rules* rules, void* stream);
+
+/* tokens[r * tokens_stride + lens[r]] = ids[r] and lens[r] += 1, for rows with
+ * live[r] > 0 (NULL: all) and 0 <= lens[r] < capacity: the tokens chosen in a
+ * step join the histories that tvr_adjust_logits reads.  A live row without
+ * room stays as it is.  tokens are int32 or int64 (token_bits 32 or 64).  No
+ * reference counterpart. */
+int tvr_history_append(void* tokens, int token_bits, int64_t tokens_stride, int32_t* lens,
+                       const int64_t* ids, const int32_t* live, int64_t rows, int64_t capacity,
+                       void* stream);
 
 /* Triangular mask of dense [batch, rows, cols]: out = x where
  * col - row >= diagonal (upper != 0, triu) or col - row <= diagonal (tril),

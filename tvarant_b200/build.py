@@ -52,6 +52,9 @@ CUDA_SOURCES = [
     "gemm_ws.cu",
     "attention.cu",
     "attention_decode.cu",
+    "paged_attention.cu",
+    "paged_ops.cu",
+    "logits.cu",
     "pointwise_jit.cu",
     "nccl.cu",
     "nvls.cu",
@@ -73,6 +76,7 @@ EXT_SOURCES = [
     "Attention.cpp",
     "Select.cpp",
     "LlamaOps.cpp",
+    "PagedOps.cpp",
 ]
 
 

@@ -31,6 +31,7 @@ ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
 BINARY_ADD, BINARY_MUL = 0, 1
 MAX_DIMS = 8
 PW_MAX_INPUTS = 16
+PAGE_F32, PAGE_F16, PAGE_BF16 = 0, 1, 2
 
 
 class TvarantError(RuntimeError):
@@ -47,6 +48,61 @@ class PwNode(ctypes.Structure):
         ("input_id", ctypes.c_int32),
         ("alpha", ctypes.c_float),
         ("c", ctypes.c_float),
+    ]
+
+
+class PagedKV(ctypes.Structure):
+    """``tvr_paged_kv``: the pages of one layer."""
+
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("page_type", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("num_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+    ]
+
+
+class PagePool(ctypes.Structure):
+    """``tvr_page_pool``: block tables and the stack of free pages."""
+
+    _fields_ = [
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("max_pages", ctypes.c_int64),
+        ("requests", ctypes.c_int64),
+        ("free_pages", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int64),
+    ]
+
+
+class LogitRules(ctypes.Structure):
+    """``tvr_logit_rules``: what ``tvr_adjust_logits`` applies."""
+
+    _fields_ = [
+        ("tokens", ctypes.c_void_p),
+        ("token_bits", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("tokens_stride", ctypes.c_int64),
+        ("prompt_lens", ctypes.c_void_p),
+        ("total_lens", ctypes.c_void_p),
+        ("repetition", ctypes.c_void_p),
+        ("presence", ctypes.c_void_p),
+        ("frequency", ctypes.c_void_p),
+        ("bias_ids", ctypes.c_void_p),
+        ("bias_values", ctypes.c_void_p),
+        ("bias_counts", ctypes.c_void_p),
+        ("bias_stride", ctypes.c_int64),
+        ("masks", ctypes.c_void_p),
+        ("mask_stride", ctypes.c_int64),
+        ("n_masks", ctypes.c_int64),
+        ("mask_rows", ctypes.c_void_p),
     ]
 
 
@@ -109,6 +165,14 @@ SIGNATURES: dict[str, list] = {
     "tvr_attention_decode_append": [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _pi64,
                                     _pi64, _pi64, _pi64, _pi64, _pi64, _f32, _vp, _i32, _vp],
     "tvr_counter_add": [_vp, _i64, _vp],
+    "tvr_page_plan": [ctypes.POINTER(PagePool), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                      _i64, _vp],
+    "tvr_paged_append": [ctypes.POINTER(PagedKV), _vp, _vp, _pi64, _vp, _i64, _vp],
+    "tvr_paged_attention": [ctypes.POINTER(PagedKV), _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
+                            _vp, _vp, _i64, _i64, _pi64, _f32, _vp, _i64, _vp],
+    "tvr_paged_attention_workspace": [_i64, _i64, _i64, _pi64],
+    "tvr_history_append": [_vp, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _vp],
+    "tvr_adjust_logits": [_vp, _i64, _vp, _i64, _i64, _i64, ctypes.POINTER(LogitRules), _vp],
     "tvr_attention_fwd": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64,
                           _pi64, _pi64, _f32, _i32, _i32, _vp],
     "tvr_bmm": [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _vp],
