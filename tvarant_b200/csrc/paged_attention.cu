@@ -3,9 +3,14 @@
 //   out[r, h] = softmax_j(scale q[r, h] . k[r, g, j]) v[r, g, j],  j < n_r,
 // with g = h / (heads / kv_heads) and n_r = seq_lens[r] read on the device.
 #include "paged_common.cuh"
+#include "tc_ptx.cuh"
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <cstring>
+#include <mutex>
+#include <type_traits>
 
 namespace tvr {
 namespace paged {
@@ -140,6 +145,1042 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
   }
 }
 
+// ---- the streaming form -------------------------------------------------------
+//
+// Bound by the stream of keys and values (2 * head_dim elements a position and
+// key head), so the work is cut by bytes, not by requests: every (request, key
+// head) is cut into tiles of kTile positions, and CTA c of G takes the tiles
+// [c N / G, (c + 1) N / G) of all N in the order request, key head, position.
+// The lengths are read on the device; nothing of this is known to the host.
+// A CTA walks through the segments of its range.  A segment that is all of its
+// (request, key head) is written out; of any other the CTA leaves maximum, sum
+// and unnormalised output in the workspace, and the last CTA to arrive at that
+// (request, key head), told by a counter, joins the parts in the order of the
+// CTAs: the result does not depend on which one was last.
+//
+// In a CTA each warp streams its own kKeys positions of every tile through a
+// ring of kStages stages in shared memory: a lane per row issues its bulk copy
+// (6.8 to 7.3 TB/s for rows of 256 bytes and more, 4.5 for 128), an mbarrier
+// per stage completes with the bytes, and a warp waits for nobody else.
+// Positions past the length, and pages out of range, are not read: their
+// scores are set to -inf and their values to zero, so that what the pages hold
+// there (NaN, infinities) does not matter.  The rows are padded so that the
+// reads below are free of bank conflicts.
+//
+// The running maximum moves only when a score exceeds it by 8 (a factor 2^8 in
+// the exp2 domain, exact after the division by the sum), so that the rescaling
+// of the outputs is rare; it starts at -FLT_MAX as in the general form.
+//
+// MT = 0, one query head a key head: DP / 16 lanes share a position, 16
+// dimensions each, fp32 FMAs.
+//
+// MT > 0, 8 MT query heads a key head: tensor cores (mma.sync with 16 rows,
+// fp32 sums), which take operands of 8 or 11 bits.  A query or weight is
+// therefore cut into terms that together carry 22 to 24 bits, each product of
+// a term with a page element is exact, and only the terms' sums are rounded:
+//   f16 pages:  x = hi + lo in f16, rows h and h + 8 of the 16.  f16 has little
+//     range, so a head's query is scaled by a power of two to 2^13 and weights
+//     by 2^7 (both are taken back exactly);
+//   bf16 pages: x = hi + mid + lo in bf16, the third in a second product;
+//   f32 pages:  x = hi + lo in tf32, and so are keys and values, their hi and
+//     lo in a product each.
+// A lane's scores are its own weights of the second product, and rows h and
+// h + 8 of a sum are in one lane: nothing is exchanged between lanes.
+constexpr int kMaxCtas = 640;  // bound on a launch's CTAs; sizes the workspace
+constexpr int kCounterBytes = 4096;
+constexpr float kSlack = 8.f;
+constexpr int kSetup = 1;
+
+template <typename T, int DP, int MT>
+struct Stream {
+  static constexpr int kElem = static_cast<int>(sizeof(T));
+  static constexpr int kChunk = 16 / kElem;        // elements of a 16-byte chunk
+  static constexpr int kRow = DP / kChunk;         // chunks of a row
+  static constexpr int kRowBytes = DP * kElem;
+  static constexpr bool kHalfs = MT > 0 && std::is_same<T, __half>::value;
+  static constexpr bool kBf16 = MT > 0 && std::is_same<T, __nv_bfloat16>::value;
+  // 4 KB a stage; for the tensor cores as many steps of 8 positions as make
+  // 8 KB, 16 at most
+  static constexpr int kKeys = MT == 0 ? 2048 / kRowBytes : kElem == 2 && DP <= 128 ? 16 : 8;
+  static constexpr int kWarps = 4;
+  static constexpr int kThreads = 32 * kWarps;
+  // by registers: 16 a lane for the output of MT = 0, MT * DP / 2 for MT > 0;
+  // and for 512-byte rows by shared memory
+  static constexpr int kCtasPerSm = MT == 0            ? 4
+                                    : kRowBytes > 512  ? 1
+                                    : MT * DP <= 128 && kRowBytes <= 256 ? 3
+                                                       : 2;
+  // Row pitches.  MT = 0: the lanes of odd rows take their chunks in another
+  // order, so that rows need no padding.  Tensor cores: 16-bit rows are read
+  // eight at a time, a chunk each; f32 keys two rows of four chunks, f32 values
+  // four even or odd rows of two.  The padding puts these on banks of their own.
+  static constexpr int kLanes = DP / 16;  // lanes of a position (MT = 0)
+  static constexpr int kPitchK = kRowBytes + (MT == 0 ? 0 : kElem == 4 ? 64 : 16);
+  static constexpr int kPitchV = kRowBytes + (MT == 0 ? 0 : 16);
+  static constexpr int kHalf = kKeys * kPitchK;  // keys, then values
+  static constexpr int kStage = kHalf + kKeys * kPitchV;
+  static constexpr int kTile = kWarps * kKeys;
+  static constexpr int kHeads = MT == 0 ? 1 : 8 * MT;
+  // query fragments of a k step of 16 (f32: 8): 16 bytes a lane, for bf16 8 more
+  static constexpr int kSteps = kElem == 4 ? DP / 8 : DP / 16;
+  static constexpr int kFrags = kBf16 ? 2 : 1;
+  static constexpr int kQueryBytes = MT * kSteps * (kBf16 ? 768 : 512);
+  static constexpr int kPartBytes = MT == 0 ? kWarps * DP * 4 : 0;  // MT > 0: in the ring
+  // as many stages as an SM's shared memory holds, four at most
+  static constexpr int kRoom = 225 * 1024 / kCtasPerSm - 384 - 512 * MT - kQueryBytes - kPartBytes;
+  static constexpr int kStages =
+      kRoom / (kWarps * kStage) < 4 ? kRoom / (kWarps * kStage) : 4;
+  static constexpr int kWarpRing = kStages * kStage;
+  static constexpr int kSmem = kWarps * kWarpRing + kQueryBytes + kPartBytes;
+  static_assert(kStages >= 2 && kKeys <= 16, "the ring");
+  static_assert(MT == 0 || kWarpRing >= kHeads * DP * 4, "a part takes the place of a ring");
+  static constexpr int kRecord = DP + 4;  // floats of one head's part: output, maximum, sum
+};
+
+struct StreamParams {
+  AttendParams a;
+  int requests;
+  int key_heads;
+  int subs;  // units of a key head: ceil(group / heads a unit)
+  int* counters;
+  float* parts;
+};
+
+using tc::smem_u32;
+
+// `bytes` (a multiple of 16) from global to shared memory, counted by `bar`.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+// Orders this thread's plain shared-memory accesses before later bulk copies.
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void lds64(uint32_t addr, uint32_t& x, uint32_t& y) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(addr));
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
+               "r"(v.z), "r"(v.w)
+               : "memory");
+}
+
+// The elements of a chunk as fp32.
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& c, float (&x)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      __half2 h;
+      memcpy(&h, &w[i], 4);
+      const float2 f = __half22float2(h);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+// fp32 values rounded to the page type, as a chunk.
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float* src) {
+  T t[16 / sizeof(T)];
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) from_f32(t[i], src[i]);
+  uint4 c;
+  memcpy(&c, t, 16);
+  return c;
+}
+
+// x = hi + lo: hi carries the leading 11 bits (rounded), which tf32 holds.
+__device__ __forceinline__ void split_rounded(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void split_cut(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// 16-bit operands, 16 or 8 products a sum.
+template <typename T>
+__device__ __forceinline__ void mma_k16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void mma_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(b0));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(b0));
+  }
+}
+
+// Four 8 x 8 matrices of 16-bit elements, lane l giving row l % 8 of matrix
+// l / 8; lane 4 g + t gets elements (g, 2 t) and (g, 2 t + 1) of each, or of
+// its transpose.
+template <bool TRANSPOSED>
+__device__ __forceinline__ uint4 ldmatrix4(uint32_t addr) {
+  uint4 v;
+  if constexpr (TRANSPOSED) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+  } else {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+  }
+  return v;
+}
+
+// Two values rounded to T, packed; x and y become what the rounding left.
+template <typename T>
+__device__ __forceinline__ uint32_t take_term(float& x, float& y) {
+  T t[2];
+  from_f32(t[0], x);
+  from_f32(t[1], y);
+  x -= to_f32(t[0]);
+  y -= to_f32(t[1]);
+  uint32_t v;
+  memcpy(&v, t, 4);
+  return v;
+}
+
+template <typename T, int DP, int MT>
+__global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>::kCtasPerSm)
+    paged_attention_stream_kernel(const __grid_constant__ StreamParams sp) {
+  using S = Stream<T, DP, MT>;
+  constexpr int CH = S::kChunk, ROW = S::kRow, KEYS = S::kKeys, HEADS = S::kHeads;
+  constexpr int WARPS = S::kWarps, THREADS = S::kThreads;
+  constexpr unsigned FULL = 0xffffffffu;
+  const AttendParams& p = sp.a;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ long long s_scan[WARPS];
+  __shared__ long long s_before;
+  __shared__ int s_request, s_last;
+  __shared__ uint32_t s_live[WARPS][S::kStages];
+  __shared__ uint64_t s_bar[WARPS][S::kStages];
+  __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_f[WARPS][HEADS];
+  __shared__ float s_top[HEADS], s_sum[HEADS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  // ---- this CTA's range of tiles
+  const int units = sp.key_heads * sp.subs;
+  auto length = [&](int r) { return max(0, min(p.max_keys, p.lens[r])); };
+  // An empty request has one tile, of no positions: somebody writes its row.
+  // A unit's first tile counts for kSetup more, what it costs to begin one.
+  auto tiles = [&](int n) { return max(1, (n + S::kTile - 1) / S::kTile) + kSetup; };
+  long long own = 0;
+  for (int r = tid; r < sp.requests; r += THREADS) own += tiles(length(r));
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) own += __shfl_xor_sync(FULL, own, x);
+  if (lane == 0) s_scan[warp] = own;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) total += s_scan[w];
+  total *= units;
+  const long long ctas = min(static_cast<long long>(gridDim.x), total);
+  const long long cta = blockIdx.x;
+  if (cta >= ctas) return;
+  long long u = cta * total / ctas;
+  const long long u_first = u, u_end = (cta + 1) * total / ctas;
+  int r, n;
+  {
+    const long long target = u / units;
+    long long before = 0;
+    for (int base = 0;; base += THREADS) {
+      __syncthreads();
+      const int q = base + tid;
+      const int t = q < sp.requests ? tiles(length(q)) : 0;
+      long long sum = t;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long below = __shfl_up_sync(FULL, sum, d);
+        if (lane >= d) sum += below;
+      }
+      if (lane == 31) s_scan[warp] = sum;
+      __syncthreads();
+      long long block = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        if (w == warp) sum += before + block;
+        block += s_scan[w];
+      }
+      if (q < sp.requests && sum > target && sum - t <= target) {
+        s_request = q;
+        s_before = sum - t;
+      }
+      before += block;
+      if (before > target) break;
+    }
+    __syncthreads();
+    r = s_request;
+    n = length(r);
+  }
+  int count = tiles(n);
+  const long long in_request = u - s_before * units;
+  int unit = static_cast<int>(in_request / count);
+  int t0 = static_cast<int>(in_request - static_cast<long long>(unit) * count);
+
+  const uint32_t ring = smem_u32(smem) + warp * S::kWarpRing;
+  const int cols = p.dim / CH;  // chunks of a row that exist
+  const uint32_t row_bytes = static_cast<uint32_t>(p.dim) * S::kElem;
+  // The padding of keys to DP dimensions has to be finite (it meets zeros of
+  // the query); values' padding ends in outputs that nobody writes.
+  auto zero_padding = [&]() {
+    if (cols == ROW) return;
+    for (int x = lane; x < S::kStages * KEYS * ROW; x += 32) {
+      const int col = x % ROW, row = x / ROW;
+      if (col >= cols) {
+        sts128(ring + (row / KEYS) * S::kStage + (row % KEYS) * S::kPitchK + col * 16,
+               make_uint4(0, 0, 0, 0));
+      }
+    }
+    fence_async();
+    __syncwarp();
+  };
+  zero_padding();
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < S::kStages; ++i) tc::mbar_init(smem_u32(&s_bar[warp][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  // The ring, over all segments: the stage to be filled, the stage to be read
+  // and the parity of its barrier.  A wait that expires (2 s) ends the filling.
+  int put = 0, get = 0;
+  uint32_t parity = 0;
+  bool failed = false;
+  float* const my_part = reinterpret_cast<float*>(
+      MT == 0 ? smem + WARPS * S::kWarpRing + S::kQueryBytes + warp * DP * 4
+              : smem + warp * S::kWarpRing);
+  constexpr int kPartStep = (MT == 0 ? DP * 4 : S::kWarpRing) / 4;  // floats between warps' parts
+  const float* const parts0 = my_part - warp * kPartStep;
+
+  while (u < u_end) {
+    const int t1 = static_cast<int>(min(static_cast<long long>(count), t0 + (u_end - u)));
+    // the tiles of the segment, without what stands for the setup; a range that
+    // ends there leaves the unit to the next CTA
+    const int real0 = max(0, t0 - kSetup), real1 = t1 - kSetup;
+    if (real1 <= 0) break;
+    const int g = unit / sp.subs, sub = unit - g * sp.subs;
+    const int h0 = g * p.group + sub * HEADS;
+    const int heads = min(HEADS, p.group - sub * HEADS);
+    const int64_t slot = p.slots != nullptr && n > 0 ? p.slots[r] : -1;
+    const int fresh = slot >= 0 && slot < p.n_slots ? n - 1 : -1;
+    if (slot >= p.n_slots && tid == 0) report(p.status, TVR_DEV_BAD_INDEX);
+
+    // ---- the ring: stage i holds this warp's positions of tile real0 + i
+    const int32_t* table = p.table + r * p.table_stride;
+    const T* kg = static_cast<const T*>(p.k) + g * p.k_s[1];
+    const T* vg = static_cast<const T*>(p.v) + g * p.v_s[1];
+    const int stages = real1 - real0;
+    const int first = real0 * S::kTile + warp * KEYS;  // the first position of stage 0
+    // Lane l copies row l % KEYS of a stage: the keys, the next KEYS lanes the
+    // values.
+    constexpr uint32_t ROWS_MASK = (1u << KEYS) - 1u;
+    const int my_row = lane % KEYS, side = lane / KEYS;
+    const T* const my_base = side == 0 ? kg : vg;
+    const int64_t page_step = side == 0 ? p.k_s[0] : p.v_s[0];
+    const int64_t row_step = side == 0 ? p.k_s[2] : p.v_s[2];
+    const uint32_t my_dst = side == 0 ? my_row * S::kPitchK : S::kHalf + my_row * S::kPitchV;
+    // the page of this lane's row in stage i, -1 if there is nothing to read
+    auto page_of = [&](int i) -> int {
+      const int j = first + i * S::kTile + my_row;
+      if (i >= stages || j >= n || j == fresh) return -1;
+      const int id = table[fast_div(static_cast<uint32_t>(j), p.page)];
+      if (id >= 0 && id < p.num_pages) return id;
+      report(p.status, TVR_DEV_BAD_INDEX);
+      return -1;
+    };
+    int filled = 0;
+    auto fill = [&](int i, int page) {
+      if (i >= stages || failed) return;
+      const uint32_t stage = ring + put * S::kStage, bar = smem_u32(&s_bar[warp][put]);
+      const int j0 = first + i * S::kTile;
+      const int new_row = fresh - j0;  // the row of the new position, if 0 <= it < KEYS
+      const bool has_new = fresh >= 0 && new_row >= 0 && new_row < KEYS;
+      const uint32_t read = __ballot_sync(FULL, page >= 0) & ROWS_MASK;
+      const uint32_t live = read | (has_new ? 1u << new_row : 0u);
+      if (lane == 0) {
+        s_live[warp][put] = live;
+        tc::mbar_expect_tx(bar, 2 * __popc(read) * row_bytes);
+      }
+      __syncwarp();
+      if (page >= 0 && side < 2) {
+        const int j = j0 + my_row;
+        const int in_page =
+            j - static_cast<int>(fast_div(static_cast<uint32_t>(j), p.page) * p.page.d);
+        bulk_copy(stage + my_dst, my_base + page * page_step + in_page * row_step, row_bytes, bar);
+      }
+      if (has_new) {
+        const float* kn = p.k_new + r * p.kn_s[0] + g * p.kn_s[1];
+        const float* vn = p.v_new + r * p.vn_s[0] + g * p.vn_s[1];
+        const int64_t pg = slot / p.page.d, in = slot - pg * p.page.d;
+        T* kc = static_cast<T*>(p.k) + pg * p.k_s[0] + g * p.k_s[1] + in * p.k_s[2];
+        T* vc = static_cast<T*>(p.v) + pg * p.v_s[0] + g * p.v_s[1] + in * p.v_s[2];
+        for (int col = lane; col < cols; col += 32) {
+          const uint4 kx = pack<T>(kn + col * CH), vx = pack<T>(vn + col * CH);
+          if (sub == 0) {
+            *reinterpret_cast<uint4*>(kc + col * CH) = kx;
+            *reinterpret_cast<uint4*>(vc + col * CH) = vx;
+          }
+          sts128(stage + new_row * S::kPitchK + col * 16, kx);
+          sts128(stage + S::kHalf + new_row * S::kPitchV + col * 16, vx);
+        }
+      }
+      if (live != ROWS_MASK) {
+        for (uint32_t dead = ~live & ROWS_MASK; dead != 0; dead &= dead - 1) {
+          const uint32_t row = stage + S::kHalf + (__ffs(dead) - 1) * S::kPitchV;
+          for (int col = lane; col < cols; col += 32) {
+            sts128(row + col * 16, make_uint4(0, 0, 0, 0));
+          }
+        }
+      }
+      if (has_new || live != ROWS_MASK) fence_async();
+      put = put + 1 == S::kStages ? 0 : put + 1;
+      ++filled;
+    };
+    // Waits for the stage to be read; false if it never comes.
+    auto ready = [&]() -> bool {
+      if (!tc::mbar_wait(smem_u32(&s_bar[warp][get]), parity, nullptr)) {
+        failed = true;
+        report(p.status, TVR_DEV_TIMEOUT_MMA);
+      }
+      failed = __any_sync(FULL, failed);
+      return !failed;
+    };
+    auto done = [&]() {
+      __syncwarp();
+      get = get + 1 == S::kStages ? 0 : get + 1;
+      parity ^= get == 0 ? 1u : 0u;
+    };
+    int pages[S::kStages];
+#pragma unroll
+    for (int i = 0; i < S::kStages; ++i) pages[i] = page_of(i);
+#pragma unroll
+    for (int i = 0; i < S::kStages; ++i) fill(i, pages[i]);
+    int next_page = page_of(S::kStages);
+
+    if constexpr (MT == 0) {
+      constexpr int L = S::kLanes, NC = 16 / CH, STEP = 32 / L;
+      const int lead = lane & (L - 1);
+      // chunk c of this lane, in the order that it reads them
+      const int turn = L < 8 ? (lane / L) & 1 : 0;
+      auto chunk = [&](int c) { return (c ^ turn) * L + lead; };
+      float q[NC][CH], o[NC][CH];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int d = chunk(c) * CH;
+        const float* src = p.q + r * p.q_s[0] + h0 * p.q_s[1] + d;
+#pragma unroll
+        for (int e = 0; e < CH; ++e) {
+          q[c][e] = d < p.dim ? src[e] * p.scale_log2 : 0.f;
+          o[c][e] = 0.f;
+        }
+      }
+      float m = -FLT_MAX, l = 0.f;  // m: one for the warp
+      for (int i = 0; i < stages && i < filled; ++i) {
+        if (!ready()) {  // what is in flight is still waited for
+          done();
+          continue;
+        }
+        const uint32_t kd = ring + get * S::kStage, vd = kd + S::kHalf;
+        const uint32_t live = s_live[warp][get];
+#pragma unroll
+        for (int it = 0; it < KEYS / STEP; ++it) {
+          const int row = it * STEP + lane / L;
+          const uint32_t rk = kd + row * S::kPitchK, rv = vd + row * S::kPitchV;
+          float s = 0.f;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            float k[CH];
+            unpack<T>(lds128(rk + chunk(c) * 16), k);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) s = fmaf(q[c][e], k[e], s);
+          }
+#pragma unroll
+          for (int x = 1; x < L; x <<= 1) s += __shfl_xor_sync(FULL, s, x);
+          s = ((live >> row) & 1u) != 0 ? s : -INFINITY;
+          if (__any_sync(FULL, s > m + kSlack)) {
+            float top = s;
+#pragma unroll
+            for (int x = L; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
+            top = fmaxf(top, m);
+            const float keep = exp2f(m - top);
+            m = top;
+            l *= keep;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+#pragma unroll
+              for (int e = 0; e < CH; ++e) o[c][e] *= keep;
+            }
+          }
+          const float w = exp2f(s - m);
+          l += w;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            float v[CH];
+            unpack<T>(lds128(rv + chunk(c) * 16), v);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) o[c][e] = fmaf(w, v[e], o[c][e]);
+          }
+        }
+        done();
+        const int ahead = i + S::kStages;
+        const int page = next_page;
+        next_page = page_of(ahead + 1);
+        fill(ahead, page);
+      }
+      // the rows' sums, lanes of even and odd rows apart as their orders differ
+      constexpr int TURNED = L < 8 ? 2 * L : L;
+#pragma unroll
+      for (int x = TURNED; x < 32; x <<= 1) {
+        l += __shfl_xor_sync(FULL, l, x);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+          for (int e = 0; e < CH; ++e) o[c][e] += __shfl_xor_sync(FULL, o[c][e], x);
+        }
+      }
+      if constexpr (L < 8) {
+        l += __shfl_xor_sync(FULL, l, L);
+        // chunk c of an even row's lane is chunk c ^ 1 of an odd row's
+#pragma unroll
+        for (int c = 0; c < NC; c += 2) {
+#pragma unroll
+          for (int e = 0; e < CH; ++e) {
+            const float a = __shfl_xor_sync(FULL, o[c][e], L);
+            const float b = __shfl_xor_sync(FULL, o[c + 1][e], L);
+            o[c][e] += b;
+            o[c + 1][e] += a;
+          }
+        }
+      }
+      if (lane < L) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+#pragma unroll
+          for (int e = 0; e < CH; ++e) my_part[chunk(c) * CH + e] = o[c][e];
+        }
+      }
+      if (lane == 0) {
+        s_m[warp][0] = m;
+        s_l[warp][0] = l;
+      }
+    } else {
+      // lane = 4 grp + thr: rows grp and grp + 8 of a fragment (head grp's terms)
+      constexpr int KS = S::kSteps, NT = KEYS / 8, MTR = MT > 0 ? MT : 1, XT = DP / 8;
+      constexpr float LIFT = S::kHalfs ? 7.f : 0.f;
+      const int grp = lane >> 2, thr = lane & 3;
+      const uint32_t query = smem_u32(smem + WARPS * S::kWarpRing) + lane * 16;
+      const uint32_t third = query + MTR * KS * 512 - lane * 8;  // bf16: the third terms
+
+      // ---- the query's fragments, shared by the warps
+      float unscale[MTR];  // f16: takes the scaling of head mt * 8 + grp back
+      if constexpr (S::kHalfs) {
+        for (int h = warp; h < HEADS; h += WARPS) {
+          float top = 0.f;
+          const float* src = p.q + r * p.q_s[0] + (h0 + h) * p.q_s[1];
+          if (h < heads) {
+            for (int d = lane; d < p.dim; d += 32) top = fmaxf(top, fabsf(src[d] * p.scale_log2));
+          }
+#pragma unroll
+          for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
+          // 2^(13 - exponent of top), within the range of fp32
+          const int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u);
+          const int lift = e == 0 || e == 255 ? 0 : max(-100, min(100, 13 - (e - 127)));
+          if (lane == 0) s_top[h] = __uint_as_float(static_cast<uint32_t>(127 + lift) << 23);
+        }
+        __syncthreads();
+      }
+      for (int x = warp; x < MTR * KS; x += WARPS) {
+        const int mt = x / KS, ks = x - mt * KS, h = mt * 8 + grp;
+        const float* src = p.q + r * p.q_s[0] + (h0 + h) * p.q_s[1];
+        const float sc = p.scale_log2 * (S::kHalfs ? s_top[h] : 1.f);
+        auto at = [&](int d) { return h < heads && d < p.dim ? src[d] * sc : 0.f; };
+        uint4 f;
+        if constexpr (sizeof(T) == 4) {
+          // step c * 2 + e takes, of chunk 4 c + thr, element 2 e as product
+          // thr and element 2 e + 1 as product thr + 4
+          const int d = (4 * (ks >> 1) + thr) * 4 + 2 * (ks & 1);
+          split_rounded(at(d), f.x, f.y);
+          split_rounded(at(d + 1), f.z, f.w);
+          sts128(query + x * 512, f);
+        } else {
+          const int d = 16 * ks + 2 * thr;
+          float a0 = at(d), a1 = at(d + 1), b0 = at(d + 8), b1 = at(d + 9);
+          f.x = take_term<T>(a0, a1);
+          f.z = take_term<T>(b0, b1);
+          f.y = take_term<T>(a0, a1);
+          f.w = take_term<T>(b0, b1);
+          sts128(query + x * 512, f);
+          if constexpr (S::kBf16) {
+            const uint32_t lo0 = take_term<T>(a0, a1), lo1 = take_term<T>(b0, b1);
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(third + x * 256), "r"(lo0),
+                         "r"(lo1)
+                         : "memory");
+          }
+        }
+      }
+      if constexpr (S::kHalfs) {
+#pragma unroll
+        for (int mt = 0; mt < MTR; ++mt) {
+          unscale[mt] = __uint_as_float((254u << 23) - __float_as_uint(s_top[mt * 8 + grp]));
+        }
+      }
+      __syncthreads();
+
+      float o[MTR][XT][4], m[MTR], l[MTR];
+#pragma unroll
+      for (int mt = 0; mt < MTR; ++mt) {
+        m[mt] = -FLT_MAX;
+        l[mt] = 0.f;
+#pragma unroll
+        for (int x = 0; x < XT; ++x) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[mt][x][e] = 0.f;
+        }
+      }
+      for (int i = 0; i < stages && i < filled; ++i) {
+        if (!ready()) {  // what is in flight is still waited for
+          done();
+          continue;
+        }
+        const uint32_t kd = ring + get * S::kStage, vd = kd + S::kHalf;
+        const uint32_t live = s_live[warp][get];
+
+        // ---- scores
+        constexpr int CHAINS = sizeof(T) == 4 ? 2 : 1;
+        float s[MTR][NT][CHAINS][4];
+#pragma unroll
+        for (int mt = 0; mt < MTR; ++mt) {
+#pragma unroll
+          for (int x = 0; x < NT * CHAINS * 4; ++x) s[mt][x / (CHAINS * 4)][x / 4 % CHAINS][x % 4] = 0.f;
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int c = 0; c < ROW / 4; ++c) {
+            float k[CH];
+            unpack<T>(lds128(kd + grp * S::kPitchK + (4 * c + thr) * 16), k);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t k0, k1, r0, r1;
+              split_cut(k[2 * e], k0, r0);
+              split_cut(k[2 * e + 1], k1, r1);
+#pragma unroll
+              for (int mt = 0; mt < MTR; ++mt) {
+                const uint4 a = lds128(query + (mt * KS + 2 * c + e) * 512);
+                mma_tf32(s[mt][0][e], a, r0, r1);
+                mma_tf32(s[mt][0][e], a, k0, k1);
+              }
+            }
+          }
+        } else {
+          const uint32_t rk = kd + (lane & 7) * S::kPitchK + (lane >> 3) * 16;
+#pragma unroll
+          for (int c = 0; c < KS / 2; ++c) {  // 32 dimensions
+            uint4 k[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              k[nt] = ldmatrix4<false>(rk + nt * 8 * S::kPitchK + c * 64);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MTR; ++mt) {
+#pragma unroll
+              for (int f = 0; f < S::kFrags; ++f) {
+                const int x = mt * KS + 2 * c;
+                uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                if (f == 0) {
+                  a = lds128(query + x * 512);
+                  b = lds128(query + x * 512 + 512);
+                } else {
+                  lds64(third + x * 256, a.x, a.z);
+                  lds64(third + x * 256 + 256, b.x, b.z);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_k16<T>(s[mt][nt][0], a, k[nt].x, k[nt].y);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_k16<T>(s[mt][nt][0], b, k[nt].z, k[nt].w);
+              }
+            }
+          }
+        }
+        // of head grp at positions 8 nt + 2 thr and the next one: the sum of
+        // the two rows of that head
+        float z[MTR][NT][2];
+        bool over = false;
+#pragma unroll
+        for (int mt = 0; mt < MTR; ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float hi = s[mt][nt][0][e], lo = s[mt][nt][0][e + 2];
+              if constexpr (CHAINS == 2) {
+                hi += s[mt][nt][1][e];
+                lo += s[mt][nt][1][e + 2];
+              }
+              float v = hi + lo;
+              if constexpr (S::kHalfs) v *= unscale[mt];
+              const bool in = ((live >> (nt * 8 + 2 * thr + e)) & 1u) != 0;
+              z[mt][nt][e] = in ? v : -INFINITY;
+              over |= z[mt][nt][e] > m[mt] + (LIFT + kSlack);
+            }
+          }
+        }
+        // m is the running maximum less LIFT: weights end below 2^(LIFT + 8)
+        if (__any_sync(FULL, over)) {
+#pragma unroll
+          for (int mt = 0; mt < MTR; ++mt) {
+            float top = z[mt][0][0];
+#pragma unroll
+            for (int x = 1; x < 2 * NT; ++x) top = fmaxf(top, z[mt][x >> 1][x & 1]);
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+            top = fmaxf(m[mt], top - LIFT);
+            const float keep = exp2f(m[mt] - top);
+            m[mt] = top;
+            l[mt] *= keep;
+#pragma unroll
+            for (int x = 0; x < XT; ++x) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[mt][x][e] *= keep;
+            }
+          }
+        }
+
+        // ---- weights, as fragments: positions 2 thr and 2 thr + 1 of each 8
+        float w[MTR][NT][2];
+#pragma unroll
+        for (int mt = 0; mt < MTR; ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            w[mt][nt][0] = exp2f(z[mt][nt][0] - m[mt]);
+            w[mt][nt][1] = exp2f(z[mt][nt][1] - m[mt]);
+            l[mt] += w[mt][nt][0] + w[mt][nt][1];
+          }
+        }
+        // ---- outputs.  The stage's products are summed on their own and then
+        // added in fp32: the tensor core cuts its running sum off below, which
+        // would show in a sum over many stages.
+        if constexpr (sizeof(T) == 4) {
+          uint4 a[MTR];
+#pragma unroll
+          for (int mt = 0; mt < MTR; ++mt) {
+            split_rounded(w[mt][0][0], a[mt].x, a[mt].y);
+            split_rounded(w[mt][0][1], a[mt].z, a[mt].w);
+          }
+          // product thr is position 2 thr, product thr + 4 the next one; tile
+          // c * 4 + e takes, of chunk 8 c + grp, element e
+          const uint32_t rv = vd + 2 * thr * S::kPitchV + grp * 16;
+#pragma unroll
+          for (int c = 0; c < ROW / 8; ++c) {
+            float v0[CH], v1[CH];
+            unpack<T>(lds128(rv + c * 128), v0);
+            unpack<T>(lds128(rv + S::kPitchV + c * 128), v1);
+#pragma unroll
+            for (int e = 0; e < CH; ++e) {
+              uint32_t x0, y0, x1, y1;
+              split_cut(v0[e], x0, y0);
+              split_cut(v1[e], x1, y1);
+#pragma unroll
+              for (int mt = 0; mt < MTR; ++mt) {
+                float t[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_tf32(t, a[mt], y0, y1);
+                mma_tf32(t, a[mt], x0, x1);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[mt][c * CH + e][x] += t[x];
+              }
+            }
+          }
+        } else {
+          uint4 a[MTR][S::kFrags];
+#pragma unroll
+          for (int mt = 0; mt < MTR; ++mt) {
+            a[mt][0].x = take_term<T>(w[mt][0][0], w[mt][0][1]);
+            a[mt][0].y = take_term<T>(w[mt][0][0], w[mt][0][1]);
+            if constexpr (S::kBf16) {
+              a[mt][S::kFrags - 1].x = take_term<T>(w[mt][0][0], w[mt][0][1]);
+              a[mt][S::kFrags - 1].y = 0;
+            }
+            if constexpr (NT == 2) {
+              a[mt][0].z = take_term<T>(w[mt][NT - 1][0], w[mt][NT - 1][1]);
+              a[mt][0].w = take_term<T>(w[mt][NT - 1][0], w[mt][NT - 1][1]);
+              if constexpr (S::kBf16) {
+                a[mt][S::kFrags - 1].z = take_term<T>(w[mt][NT - 1][0], w[mt][NT - 1][1]);
+                a[mt][S::kFrags - 1].w = 0;
+              }
+            }
+          }
+          // NT = 2: of 16 dimensions, positions 0-7 and 8-15 of the first eight,
+          // then of the next; NT = 1: eight positions of 32 dimensions
+          const uint32_t rv =
+              NT == 2 ? vd + (lane & 15) * S::kPitchV + (lane >> 4) * 16
+                      : vd + (lane & 7) * S::kPitchV + (lane >> 3) * 16;
+          constexpr int TILES = NT == 2 ? 2 : 4;
+#pragma unroll
+          for (int c = 0; c < XT / TILES; ++c) {
+            const uint4 v = ldmatrix4<true>(rv + c * TILES * 16);
+            const uint32_t vb[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int x = 0; x < TILES; ++x) {
+#pragma unroll
+              for (int mt = 0; mt < MTR; ++mt) {
+                float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int f = S::kFrags - 1; f >= 0; --f) {
+                  if constexpr (NT == 2) {
+                    mma_k16<T>(t, a[mt][f], vb[(2 * x) & 3], vb[(2 * x + 1) & 3]);
+                  } else {
+                    mma_k8<T>(t, a[mt][f].x, a[mt][f].y, vb[x]);
+                  }
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) o[mt][c * TILES + x][y] += t[y];
+              }
+            }
+          }
+        }
+        done();
+        const int ahead = i + S::kStages;
+        const int page = next_page;
+        next_page = page_of(ahead + 1);
+        fill(ahead, page);
+      }
+      // the warp's part takes the place of its ring, which is drained: every
+      // copy into it has been waited for
+#pragma unroll
+      for (int mt = 0; mt < MTR; ++mt) {
+        l[mt] += __shfl_xor_sync(FULL, l[mt], 1);
+        l[mt] += __shfl_xor_sync(FULL, l[mt], 2);
+        if (thr == 0) {
+          s_m[warp][mt * 8 + grp] = m[mt];
+          s_l[warp][mt * 8 + grp] = l[mt];
+        }
+        float* row = my_part + (mt * 8 + grp) * DP;
+#pragma unroll
+        for (int x = 0; x < XT; ++x) {
+          // the columns 2 thr and 2 thr + 1 of tile x
+          const int d = sizeof(T) == 4 ? (8 * (x / CH) + 2 * thr) * CH + x % CH : 8 * x + 2 * thr;
+          row[d] = o[mt][x][0] + o[mt][x][2];
+          row[d + (sizeof(T) == 4 ? CH : 1)] = o[mt][x][1] + o[mt][x][3];
+        }
+      }
+    }
+
+    // ---- the warps' parts into one
+    __syncthreads();
+    if (tid < HEADS) {
+      float top = -FLT_MAX, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_m[w][tid]);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = exp2f(s_m[w][tid] - top);
+        s_f[w][tid] = f;
+        sum += s_l[w][tid] * f;
+      }
+      s_top[tid] = top;
+      s_sum[tid] = sum;
+    }
+    __syncthreads();
+    const bool whole = real0 == 0 && t1 == count;
+    const long long u_unit = u - t0;  // the unit's first tile
+    float* part = sp.parts + ((2 * cta + (u == u_first ? 0 : 1)) * HEADS) * S::kRecord;
+    for (int x = tid; x < heads * DP; x += THREADS) {
+      const int h = x / DP, d = x - h * DP;
+      float acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) acc += parts0[w * kPartStep + x] * s_f[w][h];
+      if (whole) {
+        if (d < p.dim) {
+          p.out[r * p.o_s[0] + (h0 + h) * p.o_s[1] + d] = n > 0 ? acc / s_sum[h] : 0.f;
+        }
+      } else {
+        part[h * S::kRecord + d] = acc;
+      }
+    }
+    if (tid < heads) {
+      if (!whole) {
+        part[tid * S::kRecord + DP] = s_top[tid];
+        part[tid * S::kRecord + DP + 1] = s_sum[tid];
+      } else if (p.lse != nullptr) {
+        p.lse[static_cast<int64_t>(r) * p.heads + h0 + tid] =
+            n > 0 ? s_top[tid] * 0.69314718055994531f + logf(s_sum[tid]) : -INFINITY;
+      }
+    }
+    if (!whole) {
+      // CTAs of this unit: tile x belongs to CTA ((x + 1) ctas - 1) / total
+      const long long c0 = ((u_unit + kSetup + 1) * ctas - 1) / total;
+      const long long c1 = ((u_unit + count) * ctas - 1) / total;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(sp.counters + c0, 1) == static_cast<int>(c1 - c0) ? 1 : 0;
+      __syncthreads();
+      if (s_last != 0) {
+        __threadfence();
+        // c0's part is its first segment's only if the unit starts its range
+        const int late = c0 * total / ctas < u_unit ? 1 : 0;
+        const int n_parts = static_cast<int>(c1 - c0) + 1;
+        auto record = [&](int i, int h) -> const float* {
+          const long long place = 2 * (c0 + i) + (i == 0 ? late : 0);
+          return sp.parts + (place * HEADS + h) * S::kRecord;
+        };
+        for (int h = warp; h < heads; h += WARPS) {
+          float top = -FLT_MAX, sum = 0.f;
+          for (int i = lane; i < n_parts; i += 32) top = fmaxf(top, __ldcg(record(i, h) + DP));
+#pragma unroll
+          for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
+          for (int i = lane; i < n_parts; i += 32) {
+            sum += __ldcg(record(i, h) + DP + 1) * exp2f(__ldcg(record(i, h) + DP) - top);
+          }
+#pragma unroll
+          for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
+          if (lane == 0) {
+            s_top[h] = top;
+            s_sum[h] = sum;
+            if (p.lse != nullptr) {
+              p.lse[static_cast<int64_t>(r) * p.heads + h0 + h] =
+                  top * 0.69314718055994531f + logf(sum);
+            }
+          }
+        }
+        __syncthreads();
+        for (int x = tid; x < heads * DP; x += THREADS) {
+          const int h = x / DP, d = x - h * DP;
+          if (d >= p.dim) continue;
+          float acc = 0.f;
+#pragma unroll 8
+          for (int i = 0; i < n_parts; ++i) {
+            const float* rec = record(i, h);
+            acc += __ldcg(rec + d) * exp2f(__ldcg(rec + DP) - s_top[h]);
+          }
+          p.out[r * p.o_s[0] + (h0 + h) * p.o_s[1] + d] = acc / s_sum[h];
+        }
+        if (tid == 0) sp.counters[c0] = 0;
+      }
+    }
+    if constexpr (MT > 0) fence_async();
+    __syncthreads();  // the shared parts are free for the next segment
+    if constexpr (MT > 0) zero_padding();
+
+    u += t1 - t0;
+    t0 = 0;
+    if (t1 == count && ++unit == units) {
+      unit = 0;
+      ++r;
+      if (r < sp.requests) {
+        n = length(r);
+        count = tiles(n);
+      }
+    }
+  }
+}
+
+struct StreamPlan {
+  int dp = 0;  // padded head dimension; 0: the general form
+  int mt = 0;
+  int subs = 1;
+};
+
+// The padded dimension and the number of 8-head row blocks a unit takes.
+StreamPlan stream_plan(int64_t group, int64_t dim) {
+  StreamPlan s;
+  s.dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+  s.mt = group == 1 ? 0 : group <= 8 || s.dp == 256 ? 1 : 2;
+  const int64_t heads = s.mt == 0 ? 1 : 8 * s.mt;
+  s.subs = static_cast<int>(ceil_div(group, heads));
+  return s;
+}
+
+int64_t workspace_bytes_of(const StreamPlan& s) {
+  const int64_t heads = s.mt == 0 ? 1 : 8 * s.mt;
+  return kCounterBytes + 4ll * 2 * kMaxCtas * heads * (s.dp + 4);
+}
+
+template <typename T, int DP, int MT>
+int launch_stream(const StreamParams& sp, cudaStream_t stream) {
+  using S = Stream<T, DP, MT>;
+  auto kernel = paged_attention_stream_kernel<T, DP, MT>;
+  const int dev = current_device();
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  std::call_once(once[dev & 63], [&]() {
+    attr_err[dev & 63] =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  });
+  TVR_CUDA_TRY(attr_err[dev & 63]);
+  const int ctas = std::min(kMaxCtas, S::kCtasPerSm * sm_count(dev));
+  kernel<<<ctas, S::kThreads, S::kSmem, stream>>>(sp);
+  TVR_LAUNCH_CHECK();
+  return TVR_OK;
+}
+
+template <typename T>
+int launch_stream(const StreamPlan& s, const StreamParams& sp, cudaStream_t stream) {
+  switch (s.dp * 4 + s.mt) {
+    case 64 * 4: return launch_stream<T, 64, 0>(sp, stream);
+    case 64 * 4 + 1: return launch_stream<T, 64, 1>(sp, stream);
+    case 64 * 4 + 2: return launch_stream<T, 64, 2>(sp, stream);
+    case 128 * 4: return launch_stream<T, 128, 0>(sp, stream);
+    case 128 * 4 + 1: return launch_stream<T, 128, 1>(sp, stream);
+    case 128 * 4 + 2: return launch_stream<T, 128, 2>(sp, stream);
+    case 256 * 4: return launch_stream<T, 256, 0>(sp, stream);
+    default: return launch_stream<T, 256, 1>(sp, stream);
+  }
+}
+
 }  // namespace
 }  // namespace paged
 }  // namespace tvr
@@ -151,7 +1192,11 @@ extern "C" int tvr_paged_attention_workspace(int64_t heads, int64_t kv_heads, in
   TVR_CHECK(bytes != nullptr, "paged_attention_workspace: null pointer");
   TVR_CHECK(heads >= 0 && kv_heads >= 0 && head_dim >= 0 && heads <= 65535 && head_dim <= 65535,
             "paged_attention_workspace: bad size");
-  *bytes = 0;
+  TVR_CHECK(kv_heads == 0 || heads % kv_heads == 0,
+            "paged_attention_workspace: heads do not share the key heads evenly");
+  *bytes = heads == 0 || kv_heads == 0 || head_dim == 0 || head_dim > paged::kMaxDim
+               ? 0
+               : paged::workspace_bytes_of(paged::stream_plan(heads / kv_heads, head_dim));
   return TVR_OK;
 }
 
@@ -163,8 +1208,6 @@ extern "C" int tvr_paged_attention(const tvr_paged_kv* cache, const float* q, co
                                    const int64_t* strides, float scale, void* workspace,
                                    int64_t workspace_bytes, void* stream) {
   using namespace paged;
-  (void)workspace;
-  (void)workspace_bytes;
   if (int rc = check_cache(cache, "paged_attention")) return rc;
   TVR_CHECK(requests >= 0 && heads >= 0 && max_pages >= 0, "paged_attention: negative size");
   const int64_t dim = cache->head_dim;
@@ -179,7 +1222,7 @@ extern "C" int tvr_paged_attention(const tvr_paged_kv* cache, const float* q, co
             "paged_attention: k_new, v_new and slots come together");
   TVR_CHECK(table_stride >= max_pages || requests == 1,
             "paged_attention: the table's row stride is less than max_pages");
-  TVR_CHECK(max_pages <= 0x7fffffff / cache->page_size && requests * heads <= 0x7fffffff &&
+  TVR_CHECK(max_pages <= 0x7ffff000 / cache->page_size && requests * heads <= 0x7fffffff &&
                 heads <= 65535,
             "paged_attention: too many positions or heads");
   TVR_CHECK(std::isfinite(scale), "paged_attention: the scale is not finite");
@@ -218,8 +1261,36 @@ extern "C" int tvr_paged_attention(const tvr_paged_kv* cache, const float* q, co
   p.page = make_fastdiv(static_cast<uint32_t>(cache->page_size));
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = device_status_ptr(current_device());
-  const unsigned grid = static_cast<unsigned>(requests * heads);
   const cudaStream_t s = as_stream(stream);
+  // The streaming form moves 16-byte chunks: rows a whole number of them, on
+  // 16-byte boundaries.
+  const int64_t chunk = 16 / type_size(cache->page_type);
+  auto aligned = [](const void* base, const int64_t* st, int n_strides, int64_t unit) {
+    bool ok = (reinterpret_cast<uintptr_t>(base) & 15u) == 0;
+    for (int i = 0; i < n_strides; ++i) ok = ok && st[i] % unit == 0;
+    return ok;
+  };
+  if (dim % chunk == 0 && aligned(p.k, p.k_s, 3, chunk) && aligned(p.v, p.v_s, 3, chunk)) {
+    StreamParams sp = {};
+    sp.a = p;
+    sp.requests = static_cast<int>(requests);
+    sp.key_heads = static_cast<int>(cache->kv_heads);
+    const StreamPlan plan = stream_plan(p.group, dim);
+    sp.subs = plan.subs;
+    TVR_CHECK(workspace != nullptr && workspace_bytes >= workspace_bytes_of(plan),
+              "paged_attention: a workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+              (long long)workspace_bytes_of(plan));
+    TVR_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0,
+              "paged_attention: the workspace is not 16-byte aligned");
+    sp.counters = static_cast<int*>(workspace);
+    sp.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+    switch (cache->page_type) {
+      case TVR_PAGE_F32: return launch_stream<float>(plan, sp, s);
+      case TVR_PAGE_F16: return launch_stream<__half>(plan, sp, s);
+      default: return launch_stream<__nv_bfloat16>(plan, sp, s);
+    }
+  }
+  const unsigned grid = static_cast<unsigned>(requests * heads);
   switch (cache->page_type) {
     case TVR_PAGE_F32:
       paged_attention_general_kernel<float><<<grid, 32 * kGeneralWarps, 0, s>>>(p);
