@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <cmath>
 #include <cstring>
 #include <mutex>
@@ -181,7 +182,9 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
 //   f16 pages:  x = hi + lo in f16, rows h and h + 8 of the 16.  f16 has little
 //     range, so a head's query is scaled by a power of two to 2^13 and weights
 //     by 2^7 (both are taken back exactly);
-//   bf16 pages: x = hi + mid + lo in bf16, the third in a second product;
+//   bf16 pages: x = hi + mid + lo in bf16, the third in a second product; with
+//     at most four heads (PACKED) in rows h + 4 of the same one, for which a
+//     head's scores are made in two lanes, 16 apart;
 //   f32 pages:  x = hi + lo in tf32, and so are keys and values, their hi and
 //     lo in a product each.
 // A lane's scores are its own weights of the second product, and rows h and
@@ -191,7 +194,7 @@ constexpr int kCounterBytes = 4096;
 constexpr float kSlack = 8.f;
 constexpr int kSetup = 1;
 
-template <typename T, int DP, int MT>
+template <typename T, int DP, int MT, bool PACKED>
 struct Stream {
   static constexpr int kElem = static_cast<int>(sizeof(T));
   static constexpr int kChunk = 16 / kElem;        // elements of a 16-byte chunk
@@ -220,11 +223,12 @@ struct Stream {
   static constexpr int kHalf = kKeys * kPitchK;  // keys, then values
   static constexpr int kStage = kHalf + kKeys * kPitchV;
   static constexpr int kTile = kWarps * kKeys;
-  static constexpr int kHeads = MT == 0 ? 1 : 8 * MT;
+  static constexpr int kHeads = MT == 0 ? 1 : PACKED ? 4 : 8 * MT;
+  static_assert(!PACKED || (kBf16 && MT == 1), "packed rows");
   // query fragments of a k step of 16 (f32: 8): 16 bytes a lane, for bf16 8 more
   static constexpr int kSteps = kElem == 4 ? DP / 8 : DP / 16;
-  static constexpr int kFrags = kBf16 ? 2 : 1;
-  static constexpr int kQueryBytes = MT * kSteps * (kBf16 ? 768 : 512);
+  static constexpr int kFrags = kBf16 && !PACKED ? 2 : 1;
+  static constexpr int kQueryBytes = MT * kSteps * (kFrags == 2 ? 768 : 512);
   static constexpr int kPartBytes = MT == 0 ? kWarps * DP * 4 : 0;  // MT > 0: in the ring
   // as many stages as an SM's shared memory holds, four at most
   static constexpr int kRoom = 225 * 1024 / kCtasPerSm - 384 - 512 * MT - kQueryBytes - kPartBytes;
@@ -233,6 +237,11 @@ struct Stream {
   static constexpr int kWarpRing = kStages * kStage;
   static constexpr int kSmem = kWarps * kWarpRing + kQueryBytes + kPartBytes;
   static_assert(kStages >= 2 && kKeys <= 16, "the ring");
+  // the join of a unit's parts: factors and the lanes' groups' sums
+  static_assert(kWarps * kWarpRing >=
+                    4 * kHeads * (kCtasPerSm * kMaxCtas / 4 + 1 +
+                                  DP * (kHeads * DP < 128 ? kThreads * 4 / (kHeads * DP) : kWarps)),
+                "the join takes the place of the rings");
   static_assert(MT == 0 || kWarpRing >= kHeads * DP * 4, "a part takes the place of a ring");
   static constexpr int kRecord = DP + 4;  // floats of one head's part: output, maximum, sum
 };
@@ -320,47 +329,48 @@ __device__ __forceinline__ void split_cut(float x, uint32_t& hi, uint32_t& lo) {
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
+// d = a b + c, all registers; FIRST: c is zero.
+#define TVR_MMA(shape_types, a_list, b_list, ...)                                              \
+  if constexpr (FIRST) {                                                                       \
+    asm volatile("mma.sync.aligned." shape_types " {%0, %1, %2, %3}, " a_list ", " b_list      \
+                 ", {%10, %10, %10, %10};"                                                     \
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                              \
+                 : __VA_ARGS__, "f"(0.f));                                                     \
+  } else {                                                                                     \
+    asm volatile("mma.sync.aligned." shape_types " {%0, %1, %2, %3}, " a_list ", " b_list      \
+                 ", {%0, %1, %2, %3};"                                                         \
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                              \
+                 : __VA_ARGS__, "f"(0.f));                                                     \
+  }
+
+template <bool FIRST>
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+  TVR_MMA("m16n8k8.row.col.f32.tf32.tf32.f32", "{%4, %5, %6, %7}", "{%8, %9}", "r"(a.x), "r"(a.y),
+          "r"(a.z), "r"(a.w), "r"(b0), "r"(b1))
 }
 
 // 16-bit operands, 16 or 8 products a sum.
-template <typename T>
+template <typename T, bool FIRST>
 __device__ __forceinline__ void mma_k16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    TVR_MMA("m16n8k16.row.col.f32.f16.f16.f32", "{%4, %5, %6, %7}", "{%8, %9}", "r"(a.x), "r"(a.y),
+            "r"(a.z), "r"(a.w), "r"(b0), "r"(b1))
   } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    TVR_MMA("m16n8k16.row.col.f32.bf16.bf16.f32", "{%4, %5, %6, %7}", "{%8, %9}", "r"(a.x),
+            "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1))
   }
 }
-template <typename T>
-__device__ __forceinline__ void mma_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+template <typename T, bool FIRST>
+__device__ __forceinline__ void mma_k8(float (&c)[4], const uint4& a, uint32_t b0) {
   if constexpr (std::is_same<T, __half>::value) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(b0));
+    TVR_MMA("m16n8k8.row.col.f32.f16.f16.f32", "{%4, %5}", "{%8}", "r"(a.x), "r"(a.y), "r"(0),
+            "r"(0), "r"(b0), "r"(0))
   } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(b0));
+    TVR_MMA("m16n8k8.row.col.f32.bf16.bf16.f32", "{%4, %5}", "{%8}", "r"(a.x), "r"(a.y), "r"(0),
+            "r"(0), "r"(b0), "r"(0))
   }
 }
+#undef TVR_MMA
 
 // Four 8 x 8 matrices of 16-bit elements, lane l giving row l % 8 of matrix
 // l / 8; lane 4 g + t gets elements (g, 2 t) and (g, 2 t + 1) of each, or of
@@ -395,10 +405,11 @@ __device__ __forceinline__ uint32_t take_term(float& x, float& y) {
   return v;
 }
 
-template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>::kCtasPerSm)
+template <typename T, int DP, int MT, bool PACKED>
+__global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
+                                  Stream<T, DP, MT, PACKED>::kCtasPerSm)
     paged_attention_stream_kernel(const __grid_constant__ StreamParams sp) {
-  using S = Stream<T, DP, MT>;
+  using S = Stream<T, DP, MT, PACKED>;
   constexpr int CH = S::kChunk, ROW = S::kRow, KEYS = S::kKeys, HEADS = S::kHeads;
   constexpr int WARPS = S::kWarps, THREADS = S::kThreads;
   constexpr unsigned FULL = 0xffffffffu;
@@ -534,34 +545,35 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
     const int64_t page_step = side == 0 ? p.k_s[0] : p.v_s[0];
     const int64_t row_step = side == 0 ? p.k_s[2] : p.v_s[2];
     const uint32_t my_dst = side == 0 ? my_row * S::kPitchK : S::kHalf + my_row * S::kPitchV;
-    // the page of this lane's row in stage i, -1 if there is nothing to read
-    auto page_of = [&](int i) -> int {
+    // The page of this lane's row in stage i and the row in it; nothing to read
+    // where the page is negative (past the length) or out of range.
+    struct Place {
+      int page, row;
+    };
+    auto place_of = [&](int i) -> Place {
       const int j = first + i * S::kTile + my_row;
-      if (i >= stages || j >= n || j == fresh) return -1;
-      const int id = table[fast_div(static_cast<uint32_t>(j), p.page)];
-      if (id >= 0 && id < p.num_pages) return id;
-      report(p.status, TVR_DEV_BAD_INDEX);
-      return -1;
+      if (i >= stages || j >= n || j == fresh) return {INT_MIN, 0};
+      const int at = static_cast<int>(fast_div(static_cast<uint32_t>(j), p.page));
+      return {table[at], j - at * static_cast<int>(p.page.d)};
     };
     int filled = 0;
-    auto fill = [&](int i, int page) {
+    auto fill = [&](int i, const Place& place) {
       if (i >= stages || failed) return;
       const uint32_t stage = ring + put * S::kStage, bar = smem_u32(&s_bar[warp][put]);
       const int j0 = first + i * S::kTile;
       const int new_row = fresh - j0;  // the row of the new position, if 0 <= it < KEYS
       const bool has_new = fresh >= 0 && new_row >= 0 && new_row < KEYS;
-      const uint32_t read = __ballot_sync(FULL, page >= 0) & ROWS_MASK;
+      const bool in_range = static_cast<unsigned>(place.page) < static_cast<unsigned>(p.num_pages);
+      const uint32_t read = __ballot_sync(FULL, in_range) & ROWS_MASK;
       const uint32_t live = read | (has_new ? 1u << new_row : 0u);
       if (lane == 0) {
         s_live[warp][put] = live;
         tc::mbar_expect_tx(bar, 2 * __popc(read) * row_bytes);
       }
       __syncwarp();
-      if (page >= 0 && side < 2) {
-        const int j = j0 + my_row;
-        const int in_page =
-            j - static_cast<int>(fast_div(static_cast<uint32_t>(j), p.page) * p.page.d);
-        bulk_copy(stage + my_dst, my_base + page * page_step + in_page * row_step, row_bytes, bar);
+      if (in_range && side < 2) {
+        bulk_copy(stage + my_dst, my_base + place.page * page_step + place.row * row_step,
+                  row_bytes, bar);
       }
       if (has_new) {
         const float* kn = p.k_new + r * p.kn_s[0] + g * p.kn_s[1];
@@ -580,6 +592,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
         }
       }
       if (live != ROWS_MASK) {
+        if (!in_range && place.page != INT_MIN) report(p.status, TVR_DEV_BAD_INDEX);
         for (uint32_t dead = ~live & ROWS_MASK; dead != 0; dead &= dead - 1) {
           const uint32_t row = stage + S::kHalf + (__ffs(dead) - 1) * S::kPitchV;
           for (int col = lane; col < cols; col += 32) {
@@ -605,12 +618,12 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
       get = get + 1 == S::kStages ? 0 : get + 1;
       parity ^= get == 0 ? 1u : 0u;
     };
-    int pages[S::kStages];
+    Place places[S::kStages];
 #pragma unroll
-    for (int i = 0; i < S::kStages; ++i) pages[i] = page_of(i);
+    for (int i = 0; i < S::kStages; ++i) places[i] = place_of(i);
 #pragma unroll
-    for (int i = 0; i < S::kStages; ++i) fill(i, pages[i]);
-    int next_page = page_of(S::kStages);
+    for (int i = 0; i < S::kStages; ++i) fill(i, places[i]);
+    Place next = place_of(S::kStages);
 
     if constexpr (MT == 0) {
       constexpr int L = S::kLanes, NC = 16 / CH, STEP = 32 / L;
@@ -678,9 +691,9 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
         }
         done();
         const int ahead = i + S::kStages;
-        const int page = next_page;
-        next_page = page_of(ahead + 1);
-        fill(ahead, page);
+        const Place place = next;
+        next = place_of(ahead + 1);
+        fill(ahead, place);
       }
       // the rows' sums, lanes of even and odd rows apart as their orders differ
       constexpr int TURNED = L < 8 ? 2 * L : L;
@@ -745,7 +758,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
         __syncthreads();
       }
       for (int x = warp; x < MTR * KS; x += WARPS) {
-        const int mt = x / KS, ks = x - mt * KS, h = mt * 8 + grp;
+        const int mt = x / KS, ks = x - mt * KS, h = PACKED ? grp & 3 : mt * 8 + grp;
         const float* src = p.q + r * p.q_s[0] + (h0 + h) * p.q_s[1];
         const float sc = p.scale_log2 * (S::kHalfs ? s_top[h] : 1.f);
         auto at = [&](int d) { return h < heads && d < p.dim ? src[d] * sc : 0.f; };
@@ -764,8 +777,12 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
           f.z = take_term<T>(b0, b1);
           f.y = take_term<T>(a0, a1);
           f.w = take_term<T>(b0, b1);
+          if constexpr (PACKED) {
+            const uint32_t lo0 = take_term<T>(a0, a1), lo1 = take_term<T>(b0, b1);
+            if (grp >= 4) f = make_uint4(lo0, 0, lo1, 0);
+          }
           sts128(query + x * 512, f);
-          if constexpr (S::kBf16) {
+          if constexpr (S::kFrags == 2) {
             const uint32_t lo0 = take_term<T>(a0, a1), lo1 = take_term<T>(b0, b1);
             asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(third + x * 256), "r"(lo0),
                          "r"(lo1)
@@ -821,8 +838,8 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
 #pragma unroll
               for (int mt = 0; mt < MTR; ++mt) {
                 const uint4 a = lds128(query + (mt * KS + 2 * c + e) * 512);
-                mma_tf32(s[mt][0][e], a, r0, r1);
-                mma_tf32(s[mt][0][e], a, k0, k1);
+                mma_tf32<false>(s[mt][0][e], a, r0, r1);
+                mma_tf32<false>(s[mt][0][e], a, k0, k1);
               }
             }
           }
@@ -849,9 +866,9 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
                   lds64(third + x * 256 + 256, b.x, b.z);
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_k16<T>(s[mt][nt][0], a, k[nt].x, k[nt].y);
+                for (int nt = 0; nt < NT; ++nt) mma_k16<T, false>(s[mt][nt][0], a, k[nt].x, k[nt].y);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_k16<T>(s[mt][nt][0], b, k[nt].z, k[nt].w);
+                for (int nt = 0; nt < NT; ++nt) mma_k16<T, false>(s[mt][nt][0], b, k[nt].z, k[nt].w);
               }
             }
           }
@@ -873,6 +890,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
               }
               float v = hi + lo;
               if constexpr (S::kHalfs) v *= unscale[mt];
+              if constexpr (PACKED) v += __shfl_xor_sync(FULL, v, 16);
               const bool in = ((live >> (nt * 8 + 2 * thr + e)) & 1u) != 0;
               z[mt][nt][e] = in ? v : -INFINITY;
               over |= z[mt][nt][e] > m[mt] + (LIFT + kSlack);
@@ -936,9 +954,9 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
               split_cut(v1[e], x1, y1);
 #pragma unroll
               for (int mt = 0; mt < MTR; ++mt) {
-                float t[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_tf32(t, a[mt], y0, y1);
-                mma_tf32(t, a[mt], x0, x1);
+                float t[4];
+                mma_tf32<true>(t, a[mt], y0, y1);
+                mma_tf32<false>(t, a[mt], x0, x1);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) o[mt][c * CH + e][x] += t[x];
               }
@@ -951,15 +969,31 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
             a[mt][0].x = take_term<T>(w[mt][0][0], w[mt][0][1]);
             a[mt][0].y = take_term<T>(w[mt][0][0], w[mt][0][1]);
             if constexpr (S::kBf16) {
-              a[mt][S::kFrags - 1].x = take_term<T>(w[mt][0][0], w[mt][0][1]);
-              a[mt][S::kFrags - 1].y = 0;
+              const uint32_t lo = take_term<T>(w[mt][0][0], w[mt][0][1]);
+              if constexpr (PACKED) {
+                if (grp >= 4) {
+                  a[mt][0].x = lo;
+                  a[mt][0].y = 0;
+                }
+              } else {
+                a[mt][S::kFrags - 1].x = lo;
+                a[mt][S::kFrags - 1].y = 0;
+              }
             }
             if constexpr (NT == 2) {
               a[mt][0].z = take_term<T>(w[mt][NT - 1][0], w[mt][NT - 1][1]);
               a[mt][0].w = take_term<T>(w[mt][NT - 1][0], w[mt][NT - 1][1]);
               if constexpr (S::kBf16) {
-                a[mt][S::kFrags - 1].z = take_term<T>(w[mt][NT - 1][0], w[mt][NT - 1][1]);
-                a[mt][S::kFrags - 1].w = 0;
+                const uint32_t lo = take_term<T>(w[mt][NT - 1][0], w[mt][NT - 1][1]);
+                if constexpr (PACKED) {
+                  if (grp >= 4) {
+                    a[mt][0].z = lo;
+                    a[mt][0].w = 0;
+                  }
+                } else {
+                  a[mt][S::kFrags - 1].z = lo;
+                  a[mt][S::kFrags - 1].w = 0;
+                }
               }
             }
           }
@@ -977,14 +1011,15 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
             for (int x = 0; x < TILES; ++x) {
 #pragma unroll
               for (int mt = 0; mt < MTR; ++mt) {
-                float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int f = S::kFrags - 1; f >= 0; --f) {
-                  if constexpr (NT == 2) {
-                    mma_k16<T>(t, a[mt][f], vb[(2 * x) & 3], vb[(2 * x + 1) & 3]);
-                  } else {
-                    mma_k8<T>(t, a[mt][f].x, a[mt][f].y, vb[x]);
+                float t[4];
+                if constexpr (NT == 2) {
+                  mma_k16<T, true>(t, a[mt][S::kFrags - 1], vb[(2 * x) & 3], vb[(2 * x + 1) & 3]);
+                  if constexpr (S::kFrags == 2) {
+                    mma_k16<T, false>(t, a[mt][0], vb[(2 * x) & 3], vb[(2 * x + 1) & 3]);
                   }
+                } else {
+                  mma_k8<T, true>(t, a[mt][S::kFrags - 1], vb[x]);
+                  if constexpr (S::kFrags == 2) mma_k8<T, false>(t, a[mt][0], vb[x]);
                 }
 #pragma unroll
                 for (int y = 0; y < 4; ++y) o[mt][c * TILES + x][y] += t[y];
@@ -994,9 +1029,9 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
         }
         done();
         const int ahead = i + S::kStages;
-        const int page = next_page;
-        next_page = page_of(ahead + 1);
-        fill(ahead, page);
+        const Place place = next;
+        next = place_of(ahead + 1);
+        fill(ahead, place);
       }
       // the warp's part takes the place of its ring, which is drained: every
       // copy into it has been waited for
@@ -1004,7 +1039,8 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
       for (int mt = 0; mt < MTR; ++mt) {
         l[mt] += __shfl_xor_sync(FULL, l[mt], 1);
         l[mt] += __shfl_xor_sync(FULL, l[mt], 2);
-        if (thr == 0) {
+        const bool mine = !PACKED || grp < 4;
+        if (thr == 0 && mine) {
           s_m[warp][mt * 8 + grp] = m[mt];
           s_l[warp][mt * 8 + grp] = l[mt];
         }
@@ -1013,8 +1049,15 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
         for (int x = 0; x < XT; ++x) {
           // the columns 2 thr and 2 thr + 1 of tile x
           const int d = sizeof(T) == 4 ? (8 * (x / CH) + 2 * thr) * CH + x % CH : 8 * x + 2 * thr;
-          row[d] = o[mt][x][0] + o[mt][x][2];
-          row[d + (sizeof(T) == 4 ? CH : 1)] = o[mt][x][1] + o[mt][x][3];
+          float o0 = o[mt][x][0] + o[mt][x][2], o1 = o[mt][x][1] + o[mt][x][3];
+          if constexpr (PACKED) {
+            o0 += __shfl_xor_sync(FULL, o0, 16);
+            o1 += __shfl_xor_sync(FULL, o1, 16);
+          }
+          if (mine) {
+            row[d] = o0;
+            row[d + (sizeof(T) == 4 ? CH : 1)] = o1;
+          }
         }
       }
     }
@@ -1077,18 +1120,21 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
           const long long place = 2 * (c0 + i) + (i == 0 ? late : 0);
           return sp.parts + (place * HEADS + h) * S::kRecord;
         };
+        // factors [part][head] and, after them, the groups' sums: the ring is free
+        float* const s_join = reinterpret_cast<float*>(smem);
         for (int h = warp; h < heads; h += WARPS) {
           float top = -FLT_MAX, sum = 0.f;
           for (int i = lane; i < n_parts; i += 32) top = fmaxf(top, __ldcg(record(i, h) + DP));
 #pragma unroll
           for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
           for (int i = lane; i < n_parts; i += 32) {
-            sum += __ldcg(record(i, h) + DP + 1) * exp2f(__ldcg(record(i, h) + DP) - top);
+            const float f = exp2f(__ldcg(record(i, h) + DP) - top);
+            s_join[i * HEADS + h] = f;
+            sum += __ldcg(record(i, h) + DP + 1) * f;
           }
 #pragma unroll
           for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
           if (lane == 0) {
-            s_top[h] = top;
             s_sum[h] = sum;
             if (p.lse != nullptr) {
               p.lse[static_cast<int64_t>(r) * p.heads + h0 + h] =
@@ -1097,23 +1143,50 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
           }
         }
         __syncthreads();
+        // LANES lanes read a part's outputs, 16 bytes each and VECS of them;
+        // the GROUPS of lanes take the parts in turn
+        constexpr int QUADS = HEADS * DP / 4, LANES = QUADS < 32 ? QUADS : 32;
+        constexpr int VECS = QUADS / LANES, GROUPS = THREADS / LANES;
+        const int group = tid / LANES, quad = tid % LANES;
+        float acc[VECS][4];
+#pragma unroll
+        for (int v = 0; v < VECS; ++v) acc[v][0] = acc[v][1] = acc[v][2] = acc[v][3] = 0.f;
+#pragma unroll 2
+        for (int i = group; i < n_parts; i += GROUPS) {
+          const float* rec = record(i, 0);
+#pragma unroll
+          for (int v = 0; v < VECS; ++v) {
+            const int x = (v * LANES + quad) * 4, h = x / DP;
+            if (h < heads) {
+              const float4 o = __ldcg(reinterpret_cast<const float4*>(rec + x + h * 4));
+              const float f = s_join[i * HEADS + h];
+              acc[v][0] = fmaf(o.x, f, acc[v][0]);
+              acc[v][1] = fmaf(o.y, f, acc[v][1]);
+              acc[v][2] = fmaf(o.z, f, acc[v][2]);
+              acc[v][3] = fmaf(o.w, f, acc[v][3]);
+            }
+          }
+        }
+        float* const s_group = s_join + ((n_parts * HEADS + 3) & ~3);
+#pragma unroll
+        for (int v = 0; v < VECS; ++v) {
+          *reinterpret_cast<float4*>(s_group + group * HEADS * DP + (v * LANES + quad) * 4) =
+              make_float4(acc[v][0], acc[v][1], acc[v][2], acc[v][3]);
+        }
+        __syncthreads();
         for (int x = tid; x < heads * DP; x += THREADS) {
           const int h = x / DP, d = x - h * DP;
-          if (d >= p.dim) continue;
-          float acc = 0.f;
-#pragma unroll 8
-          for (int i = 0; i < n_parts; ++i) {
-            const float* rec = record(i, h);
-            acc += __ldcg(rec + d) * exp2f(__ldcg(rec + DP) - s_top[h]);
-          }
-          p.out[r * p.o_s[0] + (h0 + h) * p.o_s[1] + d] = acc / s_sum[h];
+          float sum = 0.f;
+#pragma unroll
+          for (int y = 0; y < GROUPS; ++y) sum += s_group[y * HEADS * DP + x];
+          if (d < p.dim) p.out[r * p.o_s[0] + (h0 + h) * p.o_s[1] + d] = sum / s_sum[h];
         }
         if (tid == 0) sp.counters[c0] = 0;
       }
     }
-    if constexpr (MT > 0) fence_async();
+    fence_async();
     __syncthreads();  // the shared parts are free for the next segment
-    if constexpr (MT > 0) zero_padding();
+    zero_padding();
 
     u += t1 - t0;
     t0 = 0;
@@ -1129,30 +1202,30 @@ __global__ void __launch_bounds__(Stream<T, DP, MT>::kThreads, Stream<T, DP, MT>
 }
 
 struct StreamPlan {
-  int dp = 0;  // padded head dimension; 0: the general form
-  int mt = 0;
-  int subs = 1;
+  int dp = 0;     // padded head dimension
+  int mt = 0;     // row blocks
+  int heads = 1;  // query heads of a unit
+  int subs = 1;   // units of a key head
 };
 
-// The padded dimension and the number of 8-head row blocks a unit takes.
-StreamPlan stream_plan(int64_t group, int64_t dim) {
+StreamPlan stream_plan(int page_type, int64_t group, int64_t dim) {
   StreamPlan s;
   s.dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+  // 256 dimensions leave no registers for two row blocks
   s.mt = group == 1 ? 0 : group <= 8 || s.dp == 256 ? 1 : 2;
-  const int64_t heads = s.mt == 0 ? 1 : 8 * s.mt;
-  s.subs = static_cast<int>(ceil_div(group, heads));
+  s.heads = s.mt == 0 ? 1 : page_type == TVR_PAGE_BF16 && group <= 4 ? 4 : 8 * s.mt;
+  s.subs = static_cast<int>(ceil_div(group, s.heads));
   return s;
 }
 
-int64_t workspace_bytes_of(const StreamPlan& s) {
-  const int64_t heads = s.mt == 0 ? 1 : 8 * s.mt;
-  return kCounterBytes + 4ll * 2 * kMaxCtas * heads * (s.dp + 4);
+int64_t workspace_bytes_of(int heads, int dp) {
+  return kCounterBytes + 4ll * 2 * kMaxCtas * heads * (dp + 4);
 }
 
-template <typename T, int DP, int MT>
+template <typename T, int DP, int MT, bool PACKED>
 int launch_stream(const StreamParams& sp, cudaStream_t stream) {
-  using S = Stream<T, DP, MT>;
-  auto kernel = paged_attention_stream_kernel<T, DP, MT>;
+  using S = Stream<T, DP, MT, PACKED>;
+  auto kernel = paged_attention_stream_kernel<T, DP, MT, PACKED>;
   const int dev = current_device();
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
@@ -1161,24 +1234,29 @@ int launch_stream(const StreamParams& sp, cudaStream_t stream) {
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
   });
   TVR_CUDA_TRY(attr_err[dev & 63]);
-  const int ctas = std::min(kMaxCtas, S::kCtasPerSm * sm_count(dev));
+  const int ctas = S::kCtasPerSm * std::min(kMaxCtas / 4, sm_count(dev));
   kernel<<<ctas, S::kThreads, S::kSmem, stream>>>(sp);
   TVR_LAUNCH_CHECK();
   return TVR_OK;
 }
 
+template <typename T, int DP>
+int launch_stream(const StreamPlan& s, const StreamParams& sp, cudaStream_t stream) {
+  if (s.mt == 0) return launch_stream<T, DP, 0, false>(sp, stream);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    if (s.heads == 4) return launch_stream<T, DP, 1, true>(sp, stream);
+  }
+  if constexpr (DP < 256) {
+    if (s.mt == 2) return launch_stream<T, DP, 2, false>(sp, stream);
+  }
+  return launch_stream<T, DP, 1, false>(sp, stream);
+}
+
 template <typename T>
 int launch_stream(const StreamPlan& s, const StreamParams& sp, cudaStream_t stream) {
-  switch (s.dp * 4 + s.mt) {
-    case 64 * 4: return launch_stream<T, 64, 0>(sp, stream);
-    case 64 * 4 + 1: return launch_stream<T, 64, 1>(sp, stream);
-    case 64 * 4 + 2: return launch_stream<T, 64, 2>(sp, stream);
-    case 128 * 4: return launch_stream<T, 128, 0>(sp, stream);
-    case 128 * 4 + 1: return launch_stream<T, 128, 1>(sp, stream);
-    case 128 * 4 + 2: return launch_stream<T, 128, 2>(sp, stream);
-    case 256 * 4: return launch_stream<T, 256, 0>(sp, stream);
-    default: return launch_stream<T, 256, 1>(sp, stream);
-  }
+  if (s.dp == 64) return launch_stream<T, 64>(s, sp, stream);
+  if (s.dp == 128) return launch_stream<T, 128>(s, sp, stream);
+  return launch_stream<T, 256>(s, sp, stream);
 }
 
 }  // namespace
@@ -1194,9 +1272,12 @@ extern "C" int tvr_paged_attention_workspace(int64_t heads, int64_t kv_heads, in
             "paged_attention_workspace: bad size");
   TVR_CHECK(kv_heads == 0 || heads % kv_heads == 0,
             "paged_attention_workspace: heads do not share the key heads evenly");
-  *bytes = heads == 0 || kv_heads == 0 || head_dim == 0 || head_dim > paged::kMaxDim
-               ? 0
-               : paged::workspace_bytes_of(paged::stream_plan(heads / kv_heads, head_dim));
+  *bytes = 0;
+  if (heads > 0 && kv_heads > 0 && head_dim > 0 && head_dim <= paged::kMaxDim) {
+    // whatever the pages' type: f32 and f16 units are the largest
+    const paged::StreamPlan s = paged::stream_plan(TVR_PAGE_F32, heads / kv_heads, head_dim);
+    *bytes = paged::workspace_bytes_of(s.heads, s.dp);
+  }
   return TVR_OK;
 }
 
@@ -1275,11 +1356,12 @@ extern "C" int tvr_paged_attention(const tvr_paged_kv* cache, const float* q, co
     sp.a = p;
     sp.requests = static_cast<int>(requests);
     sp.key_heads = static_cast<int>(cache->kv_heads);
-    const StreamPlan plan = stream_plan(p.group, dim);
+    const StreamPlan plan = stream_plan(cache->page_type, p.group, dim);
+    const int64_t need = workspace_bytes_of(plan.heads, plan.dp);
     sp.subs = plan.subs;
-    TVR_CHECK(workspace != nullptr && workspace_bytes >= workspace_bytes_of(plan),
+    TVR_CHECK(workspace != nullptr && workspace_bytes >= need,
               "paged_attention: a workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
-              (long long)workspace_bytes_of(plan));
+              (long long)need);
     TVR_CHECK((reinterpret_cast<uintptr_t>(workspace) & 15u) == 0,
               "paged_attention: the workspace is not 16-byte aligned");
     sp.counters = static_cast<int*>(workspace);
