@@ -535,7 +535,7 @@ typedef struct tvr_logit_rules {
 } tvr_logit_rules;
 
 /* out[r, v] = logits[r, v] adjusted, in this order:
- *   token v in row r's history:  l = l > 0 ? l / repetition : l * repetition
+ *   token v in row r's history:  l = l * (l > 0 ? 1 / repetition : repetition)
  *   c times among the generated: l = l - frequency * c, then - presence if c
  *   biases of token v:           l = l + value, in the order of the list
  *   token v not allowed:         l = -inf, whatever the above gave

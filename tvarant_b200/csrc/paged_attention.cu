@@ -324,10 +324,6 @@ __device__ __forceinline__ void split_rounded(float x, uint32_t& hi, uint32_t& l
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
-__device__ __forceinline__ void split_cut(float x, uint32_t& hi, uint32_t& lo) {
-  hi = __float_as_uint(x) & 0xffffe000u;
-  lo = __float_as_uint(x - __uint_as_float(hi));
-}
 
 // d = a b + c, all registers; FIRST: c is zero.
 #define TVR_MMA(shape_types, a_list, b_list, ...)                                              \
@@ -833,8 +829,8 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               uint32_t k0, k1, r0, r1;
-              split_cut(k[2 * e], k0, r0);
-              split_cut(k[2 * e + 1], k1, r1);
+              split_rounded(k[2 * e], k0, r0);
+              split_rounded(k[2 * e + 1], k1, r1);
 #pragma unroll
               for (int mt = 0; mt < MTR; ++mt) {
                 const uint4 a = lds128(query + (mt * KS + 2 * c + e) * 512);
@@ -950,8 +946,8 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
 #pragma unroll
             for (int e = 0; e < CH; ++e) {
               uint32_t x0, y0, x1, y1;
-              split_cut(v0[e], x0, y0);
-              split_cut(v1[e], x1, y1);
+              split_rounded(v0[e], x0, y0);
+              split_rounded(v1[e], x1, y1);
 #pragma unroll
               for (int mt = 0; mt < MTR; ++mt) {
                 float t[4];

@@ -5,6 +5,7 @@
 #include "cluster.cuh"
 
 #include <climits>
+#include <cstring>
 
 namespace tvr {
 namespace paged {
@@ -232,8 +233,11 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const __grid_constant__
 // ---- append -------------------------------------------------------------------
 //
 // A copy with conversion: reads 4 bytes and writes 4 or 2 per value, bound by
-// memory.  A thread moves VEC values (16 bytes of a page row where the
-// operands allow it), the threads of a token side by side.
+// memory.  A thread moves VEC values, 16 bytes of a page row where the
+// operands allow it (one value where they do not), kBatch of them under way;
+// the threads of a token lie side by side.
+constexpr int kBatch = 2;
+
 struct AppendParams {
   void* pages[2];
   const float* src[2];
@@ -241,7 +245,7 @@ struct AppendParams {
   int64_t src_stride[2][2];   // token, head
   const int64_t* slots;
   int64_t n_slots;  // num_pages * page_size
-  int64_t page_size;
+  FastDiv page_size;
   int64_t items;
   FastDiv per_token, per_side, per_head;  // vectors of a token (K and V), of one side, of a head
   int* status;
@@ -250,28 +254,63 @@ struct AppendParams {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ AppendParams p) {
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; item < p.items;
-       item += step) {
-    const int64_t token = item <= UINT_MAX
-                              ? fast_div(static_cast<uint32_t>(item), p.per_token)
-                              : item / p.per_token.d;
-    const uint32_t in_token = static_cast<uint32_t>(item - token * p.per_token.d);
-    const uint32_t side = fast_div(in_token, p.per_side);
-    const uint32_t in_side = in_token - side * p.per_side.d;
-    const uint32_t head = fast_div(in_side, p.per_head);
-    const uint32_t d = (in_side - head * p.per_head.d) * VEC;
-    const int64_t slot = p.slots[token];
-    if (slot < 0) continue;
-    if (slot >= p.n_slots) {
-      if (in_token == 0) report(p.status, TVR_DEV_BAD_INDEX);
-      continue;
-    }
-    const int64_t page = slot / p.page_size, at = slot - page * p.page_size;
-    const float* src = p.src[side] + token * p.src_stride[side][0] + head * p.src_stride[side][1] + d;
-    T* dst = static_cast<T*>(p.pages[side]) + page * p.page_stride[side][0] +
-             head * p.page_stride[side][1] + at * p.page_stride[side][2] + d;
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+       first < p.items; first += kBatch * step) {
+    float x[kBatch][VEC];
+    T* dst[kBatch];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) from_f32(dst[i], src[i]);
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t item = first + b * step;
+      dst[b] = nullptr;
+      if (item >= p.items) continue;
+      const int64_t token = item <= UINT_MAX
+                                ? fast_div(static_cast<uint32_t>(item), p.per_token)
+                                : item / p.per_token.d;
+      const uint32_t in_token = static_cast<uint32_t>(item - token * p.per_token.d);
+      const uint32_t side = fast_div(in_token, p.per_side);
+      const uint32_t in_side = in_token - side * p.per_side.d;
+      const uint32_t head = fast_div(in_side, p.per_head);
+      const uint32_t d = (in_side - head * p.per_head.d) * VEC;
+      const float* src =
+          p.src[side] + token * p.src_stride[side][0] + head * p.src_stride[side][1] + d;
+      if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+          const float4 v = __ldg(reinterpret_cast<const float4*>(src + i));
+          x[b][i] = v.x;
+          x[b][i + 1] = v.y;
+          x[b][i + 2] = v.z;
+          x[b][i + 3] = v.w;
+        }
+      } else {
+        x[b][0] = __ldg(src);
+      }
+      const int64_t slot = __ldg(p.slots + token);
+      if (slot < 0) continue;
+      if (slot >= p.n_slots) {
+        if (in_token == 0) report(p.status, TVR_DEV_BAD_INDEX);
+        continue;
+      }
+      const int64_t page = slot <= UINT_MAX ? fast_div(static_cast<uint32_t>(slot), p.page_size)
+                                            : slot / p.page_size.d;
+      const int64_t at = slot - page * p.page_size.d;
+      dst[b] = static_cast<T*>(p.pages[side]) + page * p.page_stride[side][0] +
+               head * p.page_stride[side][1] + at * p.page_stride[side][2] + d;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (dst[b] == nullptr) continue;
+      T t[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) from_f32(t[i], x[b][i]);
+      if constexpr (VEC == 1) {
+        *dst[b] = t[0];
+      } else {
+        uint4 v;
+        memcpy(&v, t, 16);
+        *reinterpret_cast<uint4*>(dst[b]) = v;
+      }
+    }
   }
 }
 
@@ -283,9 +322,23 @@ int append(AppendParams& p, int64_t tokens, int64_t heads, int64_t dim, cudaStre
   p.per_token = make_fastdiv(static_cast<uint32_t>(2 * per_head * heads));
   p.items = tokens * 2 * per_head * heads;
   paged_append_kernel<T, VEC>
-      <<<elementwise_grid(p.items, 256, current_device()), 256, 0, stream>>>(p);
+      <<<elementwise_grid(ceil_div(p.items, kBatch), 256, current_device()), 256, 0, stream>>>(p);
   TVR_LAUNCH_CHECK();
   return TVR_OK;
+}
+
+template <typename T>
+int append(AppendParams& p, int64_t tokens, int64_t heads, int64_t dim, cudaStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T);
+  bool whole = dim % VEC == 0;
+  for (int side = 0; side < 2; ++side) {
+    whole = whole && reinterpret_cast<uintptr_t>(p.pages[side]) % 16 == 0 &&
+            reinterpret_cast<uintptr_t>(p.src[side]) % 16 == 0;
+    for (int64_t st : p.page_stride[side]) whole = whole && st % VEC == 0;
+    for (int64_t st : p.src_stride[side]) whole = whole && st % 4 == 0;
+  }
+  return whole ? append<T, VEC>(p, tokens, heads, dim, stream)
+               : append<T, 1>(p, tokens, heads, dim, stream);
 }
 
 }  // namespace
@@ -392,11 +445,11 @@ extern "C" int tvr_paged_append(const tvr_paged_kv* cache, const float* k_new, c
   }
   p.slots = slots;
   p.n_slots = cache->num_pages * cache->page_size;
-  p.page_size = cache->page_size;
+  p.page_size = make_fastdiv(static_cast<uint32_t>(cache->page_size));
   p.status = device_status_ptr(current_device());
   switch (cache->page_type) {
-    case TVR_PAGE_F32: return append<float, 1>(p, tokens, heads, dim, as_stream(stream));
-    case TVR_PAGE_F16: return append<__half, 1>(p, tokens, heads, dim, as_stream(stream));
-    default: return append<__nv_bfloat16, 1>(p, tokens, heads, dim, as_stream(stream));
+    case TVR_PAGE_F32: return append<float>(p, tokens, heads, dim, as_stream(stream));
+    case TVR_PAGE_F16: return append<__half>(p, tokens, heads, dim, as_stream(stream));
+    default: return append<__nv_bfloat16>(p, tokens, heads, dim, as_stream(stream));
   }
 }
