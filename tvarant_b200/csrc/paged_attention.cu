@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
 constexpr int kMaxCtas = 640;  // bound on a launch's CTAs; sizes the workspace
 constexpr int kCounterBytes = 4096;
 constexpr float kSlack = 8.f;
-constexpr int kSetup = 1;
+constexpr int kSetup = 3;
 
 template <typename T, int DP, int MT, bool PACKED>
 struct Stream {
@@ -200,7 +200,7 @@ struct Stream {
   static constexpr int kChunk = 16 / kElem;        // elements of a 16-byte chunk
   static constexpr int kRow = DP / kChunk;         // chunks of a row
   static constexpr int kRowBytes = DP * kElem;
-  static constexpr bool kHalfs = MT > 0 && std::is_same<T, __half>::value;
+  [[maybe_unused]] static constexpr bool kHalfs = MT > 0 && std::is_same<T, __half>::value;
   static constexpr bool kBf16 = MT > 0 && std::is_same<T, __nv_bfloat16>::value;
   // 4 KB a stage; for the tensor cores as many steps of 8 positions as make
   // 8 KB, 16 at most
@@ -217,7 +217,7 @@ struct Stream {
   // order, so that rows need no padding.  Tensor cores: 16-bit rows are read
   // eight at a time, a chunk each; f32 keys two rows of four chunks, f32 values
   // four even or odd rows of two.  The padding puts these on banks of their own.
-  static constexpr int kLanes = DP / 16;  // lanes of a position (MT = 0)
+  [[maybe_unused]] static constexpr int kLanes = DP / 16;  // lanes of a position (MT = 0)
   static constexpr int kPitchK = kRowBytes + (MT == 0 ? 0 : kElem == 4 ? 64 : 16);
   static constexpr int kPitchV = kRowBytes + (MT == 0 ? 0 : 16);
   static constexpr int kHalf = kKeys * kPitchK;  // keys, then values
