@@ -160,13 +160,13 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
 // CTAs: the result does not depend on which one was last.
 //
 // In a CTA each warp streams its own kKeys positions of every tile through a
-// ring of kStages stages in shared memory: a lane per row issues its bulk copy
-// (6.8 to 7.3 TB/s for rows of 256 bytes and more, 4.5 for 128), an mbarrier
-// per stage completes with the bytes, and a warp waits for nobody else.
-// Positions past the length, and pages out of range, are not read: their
-// scores are set to -inf and their values to zero, so that what the pages hold
-// there (NaN, infinities) does not matter.  The rows are padded so that the
-// reads below are free of bank conflicts.
+// ring of kStages stages in shared memory (16-byte cp.async; a warp waits for
+// nobody else).  Bulk copies of whole rows carry the same bytes with fewer
+// instructions, but a warp issues one in 80 cycles, 1300 to 2600 for a stage,
+// which is what bounded short requests.  Positions past the length, and pages
+// out of range, are filled with zeros instead of read, and their scores set to
+// -inf, so that what the pages hold there (NaN, infinities) does not matter.
+// The rows are padded so that the reads below are free of bank conflicts.
 //
 // The running maximum moves only when a score exceeds it by 8 (a factor 2^8 in
 // the exp2 domain, exact after the division by the sum), so that the rescaling
@@ -200,7 +200,6 @@ struct Stream {
   static constexpr int kChunk = 16 / kElem;        // elements of a 16-byte chunk
   static constexpr int kRow = DP / kChunk;         // chunks of a row
   static constexpr int kRowBytes = DP * kElem;
-  [[maybe_unused]] static constexpr bool kHalfs = MT > 0 && std::is_same<T, __half>::value;
   static constexpr bool kBf16 = MT > 0 && std::is_same<T, __nv_bfloat16>::value;
   // 4 KB a stage; for the tensor cores as many steps of 8 positions as make
   // 8 KB, 16 at most
@@ -217,7 +216,6 @@ struct Stream {
   // order, so that rows need no padding.  Tensor cores: 16-bit rows are read
   // eight at a time, a chunk each; f32 keys two rows of four chunks, f32 values
   // four even or odd rows of two.  The padding puts these on banks of their own.
-  [[maybe_unused]] static constexpr int kLanes = DP / 16;  // lanes of a position (MT = 0)
   static constexpr int kPitchK = kRowBytes + (MT == 0 ? 0 : kElem == 4 ? 64 : 16);
   static constexpr int kPitchV = kRowBytes + (MT == 0 ? 0 : 16);
   static constexpr int kHalf = kKeys * kPitchK;  // keys, then values
@@ -229,20 +227,18 @@ struct Stream {
   static constexpr int kSteps = kElem == 4 ? DP / 8 : DP / 16;
   static constexpr int kFrags = kBf16 && !PACKED ? 2 : 1;
   static constexpr int kQueryBytes = MT * kSteps * (kFrags == 2 ? 768 : 512);
-  static constexpr int kPartBytes = MT == 0 ? kWarps * DP * 4 : 0;  // MT > 0: in the ring
+  // MT = 0: the warps' parts, or the sums of eight groups of lanes that join a
+  // unit's parts; MT > 0: in the ring
+  static constexpr int kPartBytes = MT == 0 ? (DP == 64 ? 8 : 4) * DP * 4 : 0;
   // as many stages as an SM's shared memory holds, four at most
-  static constexpr int kRoom = 225 * 1024 / kCtasPerSm - 384 - 512 * MT - kQueryBytes - kPartBytes;
+  static constexpr int kRoom = 225 * 1024 / kCtasPerSm - (MT == 2 ? 1792 : 1024) - kQueryBytes -
+                               kPartBytes;
   static constexpr int kStages =
       kRoom / (kWarps * kStage) < 4 ? kRoom / (kWarps * kStage) : 4;
   static constexpr int kWarpRing = kStages * kStage;
   static constexpr int kSmem = kWarps * kWarpRing + kQueryBytes + kPartBytes;
   static_assert(kStages >= 2 && kKeys <= 16, "the ring");
-  // the join of a unit's parts: factors and the lanes' groups' sums
-  static_assert(kWarps * kWarpRing >=
-                    4 * kHeads * (kCtasPerSm * kMaxCtas / 4 + 1 +
-                                  DP * (kHeads * DP < 128 ? kThreads * 4 / (kHeads * DP) : kWarps)),
-                "the join takes the place of the rings");
-  static_assert(MT == 0 || kWarpRing >= kHeads * DP * 4, "a part takes the place of a ring");
+  static_assert(MT == 0 || kStage >= kHeads * (DP + 8) * 4, "a part takes the place of a stage");
   static constexpr int kRecord = DP + 4;  // floats of one head's part: output, maximum, sum
 };
 
@@ -257,20 +253,21 @@ struct StreamParams {
 
 using tc::smem_u32;
 
-// `bytes` (a multiple of 16) from global to shared memory, counted by `bar`.
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
+// 16 bytes from global to shared memory; or 16 zeros, with nothing read.
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// Orders this thread's plain shared-memory accesses before later bulk copies.
-__device__ __forceinline__ void fence_async() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+__device__ __forceinline__ void copy_async_or_zero(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(live ? 16 : 0)
+               : "memory");
 }
-
+// N bytes (4 or 8) from global to shared memory, waited for by cp.async.wait_all.
+template <int N>
+__device__ __forceinline__ void fetch_async(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(N)
+               : "memory");
+}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -281,10 +278,26 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 __device__ __forceinline__ void lds64(uint32_t addr, uint32_t& x, uint32_t& y) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(addr));
 }
+__device__ __forceinline__ void sts64(uint32_t addr, uint32_t x, uint32_t y) {
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(addr), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
                "r"(v.z), "r"(v.w)
                : "memory");
+}
+
+// dst[0 .. 3] = x f, in one store where dst allows it.
+__device__ __forceinline__ void put_four(float* dst, const float4& x, float f) {
+  const float4 y = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+  if ((reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+    *reinterpret_cast<float4*>(dst) = y;
+  } else {
+    dst[0] = y.x;
+    dst[1] = y.y;
+    dst[2] = y.z;
+    dst[3] = y.w;
+  }
 }
 
 // The elements of a chunk as fp32.
@@ -409,15 +422,15 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
   constexpr int CH = S::kChunk, ROW = S::kRow, KEYS = S::kKeys, HEADS = S::kHeads;
   constexpr int WARPS = S::kWarps, THREADS = S::kThreads;
   constexpr unsigned FULL = 0xffffffffu;
+  [[maybe_unused]] constexpr bool HALFS = std::is_same<T, __half>::value;
   const AttendParams& p = sp.a;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long s_scan[WARPS];
   __shared__ long long s_before;
   __shared__ int s_request, s_last;
   __shared__ uint32_t s_live[WARPS][S::kStages];
-  __shared__ uint64_t s_bar[WARPS][S::kStages];
   __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_f[WARPS][HEADS];
-  __shared__ float s_top[HEADS], s_sum[HEADS];
+  __shared__ float s_top[HEADS], s_sum[HEADS], s_inverse[HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   // ---- this CTA's range of tiles
@@ -426,49 +439,63 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
   // An empty request has one tile, of no positions: somebody writes its row.
   // A unit's first tile counts for kSetup more, what it costs to begin one.
   auto tiles = [&](int n) { return max(1, (n + S::kTile - 1) / S::kTile) + kSetup; };
-  long long own = 0;
-  for (int r = tid; r < sp.requests; r += THREADS) own += tiles(length(r));
+  // The first THREADS requests' inclusive sums are kept; further ones are only
+  // summed, and scanned below where the range begins among them.
+  auto scan = [&](long long x) -> long long {  // inclusive, over the CTA
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) own += __shfl_xor_sync(FULL, own, x);
-  if (lane == 0) s_scan[warp] = own;
-  __syncthreads();
-  long long total = 0;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long below = __shfl_up_sync(FULL, x, d);
+      if (lane >= d) x += below;
+    }
+    if (lane == 31) s_scan[warp] = x;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) total += s_scan[w];
+    for (int w = 0; w < WARPS - 1; ++w) x += w < warp ? s_scan[w] : 0;
+    return x;
+  };
+  const int my_tiles = tid < sp.requests ? tiles(length(tid)) : 0;
+  const long long my_end = scan(my_tiles);
+  long long head_tiles = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) head_tiles += s_scan[w];
+  total = head_tiles;
+  if (sp.requests > THREADS) {
+    long long own = 0;
+    for (int q = THREADS + tid; q < sp.requests; q += THREADS) own += tiles(length(q));
+    __syncthreads();
+    own = scan(own);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += s_scan[w];
+  }
   total *= units;
   const long long ctas = min(static_cast<long long>(gridDim.x), total);
   const long long cta = blockIdx.x;
   if (cta >= ctas) return;
-  long long u = cta * total / ctas;
-  const long long u_first = u, u_end = (cta + 1) * total / ctas;
+  // tile x belongs to CTA ((x + 1) ctas - 1) / total; CTA c begins at c total / ctas
+  auto divide = [](long long x, long long y) -> long long {  // x, y >= 0
+    return ((x | y) >> 32) == 0 ? static_cast<uint32_t>(x) / static_cast<uint32_t>(y) : x / y;
+  };
+  long long u = divide(cta * total, ctas);
+  const long long u_first = u, u_end = divide((cta + 1) * total, ctas);
   int r, n;
   {
-    const long long target = u / units;
-    long long before = 0;
-    for (int base = 0;; base += THREADS) {
+    const long long target = divide(u, units);
+    if (my_tiles > 0 && my_end > target && my_end - my_tiles <= target) {
+      s_request = tid;
+      s_before = my_end - my_tiles;
+    }
+    long long before = head_tiles;
+    for (int base = THREADS; before <= target; base += THREADS) {
       __syncthreads();
       const int q = base + tid;
       const int t = q < sp.requests ? tiles(length(q)) : 0;
-      long long sum = t;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long below = __shfl_up_sync(FULL, sum, d);
-        if (lane >= d) sum += below;
-      }
-      if (lane == 31) s_scan[warp] = sum;
-      __syncthreads();
-      long long block = 0;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        if (w == warp) sum += before + block;
-        block += s_scan[w];
-      }
-      if (q < sp.requests && sum > target && sum - t <= target) {
+      const long long end = before + scan(t);
+      if (q < sp.requests && end > target && end - t <= target) {
         s_request = q;
-        s_before = sum - t;
+        s_before = end - t;
       }
-      before += block;
-      if (before > target) break;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) before += s_scan[w];
     }
     __syncthreads();
     r = s_request;
@@ -476,153 +503,205 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
   }
   int count = tiles(n);
   const long long in_request = u - s_before * units;
-  int unit = static_cast<int>(in_request / count);
+  int unit = static_cast<int>(divide(in_request, count));
   int t0 = static_cast<int>(in_request - static_cast<long long>(unit) * count);
 
   const uint32_t ring = smem_u32(smem) + warp * S::kWarpRing;
   const int cols = p.dim / CH;  // chunks of a row that exist
-  const uint32_t row_bytes = static_cast<uint32_t>(p.dim) * S::kElem;
-  // The padding of keys to DP dimensions has to be finite (it meets zeros of
-  // the query); values' padding ends in outputs that nobody writes.
-  auto zero_padding = [&]() {
-    if (cols == ROW) return;
-    for (int x = lane; x < S::kStages * KEYS * ROW; x += 32) {
-      const int col = x % ROW, row = x / ROW;
-      if (col >= cols) {
-        sts128(ring + (row / KEYS) * S::kStage + (row % KEYS) * S::kPitchK + col * 16,
-               make_uint4(0, 0, 0, 0));
-      }
-    }
-    fence_async();
-    __syncwarp();
-  };
-  zero_padding();
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < S::kStages; ++i) tc::mbar_init(smem_u32(&s_bar[warp][i]), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncwarp();
-  // The ring, over all segments: the stage to be filled, the stage to be read
-  // and the parity of its barrier.  A wait that expires (2 s) ends the filling.
+  // pages hold whole stages
+  const bool aligned = (p.page.d & (KEYS - 1)) == 0 && cols == ROW;
+  // The ring, over all segments: the stage to be filled, the stage to be read.
   int put = 0, get = 0;
-  uint32_t parity = 0;
-  bool failed = false;
-  float* const my_part = reinterpret_cast<float*>(
-      MT == 0 ? smem + WARPS * S::kWarpRing + S::kQueryBytes + warp * DP * 4
-              : smem + warp * S::kWarpRing);
-  constexpr int kPartStep = (MT == 0 ? DP * 4 : S::kWarpRing) / 4;  // floats between warps' parts
-  const float* const parts0 = my_part - warp * kPartStep;
+  // Where a warp leaves its part of a segment: MT = 0, in a place of its own;
+  // MT > 0, in the stage of its ring that is filled last.
+  auto part_of = [&](int w) -> float* {
+    if constexpr (MT == 0) {
+      return reinterpret_cast<float*>(smem + WARPS * S::kWarpRing) + w * DP;
+    } else {
+      const int stage = put == 0 ? S::kStages - 1 : put - 1;
+      return reinterpret_cast<float*>(smem + w * S::kWarpRing + stage * S::kStage);
+    }
+  };
+  constexpr int PART = MT == 0 ? DP : DP + 8;  // floats from one head of a part to the next
+  // Stages that are filled before the parts of the segment before are joined;
+  // what that takes (length, slot, pages) is fetched during that segment.
+  constexpr int EARLY = MT == 0 ? S::kStages : S::kStages - 1;
+  __shared__ int s_pages[WARPS][EARLY][KEYS], s_length[WARPS];
+  __shared__ int64_t s_slot[WARPS];
 
-  while (u < u_end) {
-    const int t1 = static_cast<int>(min(static_cast<long long>(count), t0 + (u_end - u)));
-    // the tiles of the segment, without what stands for the setup; a range that
-    // ends there leaves the unit to the next CTA
-    const int real0 = max(0, t0 - kSetup), real1 = t1 - kSetup;
-    if (real1 <= 0) break;
-    const int g = unit / sp.subs, sub = unit - g * sp.subs;
-    const int h0 = g * p.group + sub * HEADS;
-    const int heads = min(HEADS, p.group - sub * HEADS);
-    const int64_t slot = p.slots != nullptr && n > 0 ? p.slots[r] : -1;
-    const int fresh = slot >= 0 && slot < p.n_slots ? n - 1 : -1;
-    if (slot >= p.n_slots && tid == 0) report(p.status, TVR_DEV_BAD_INDEX);
+  // ---- the segment at hand: positions of (request r, unit), tiles real0 to
+  // real1 without what stands for the setup; a range that ends there leaves the
+  // unit to the next CTA
+  int t1 = 0, real0 = 0, stages = 0, first = 0, fresh = -1, g = 0, sub = 0;
+  int64_t slot = -1;
+  auto slot_of = [&](int q) -> int64_t { return p.slots != nullptr ? p.slots[q] : -1; };
+  // the rest of the segment's numbers; false if it has no tiles
+  auto begin = [&]() -> bool {
+    t1 = static_cast<int>(min(static_cast<long long>(count), t0 + (u_end - u)));
+    real0 = max(0, t0 - kSetup);
+    stages = t1 - kSetup - real0;
+    first = real0 * S::kTile + warp * KEYS;  // the warp's first position of stage 0
+    g = unit / sp.subs;
+    sub = unit - g * sp.subs;
+    fresh = n > 0 && slot >= 0 && slot < p.n_slots ? n - 1 : -1;
+    if (n > 0 && slot >= p.n_slots && tid == 0) report(p.status, TVR_DEV_BAD_INDEX);
+    return t1 > kSetup;
+  };
 
-    // ---- the ring: stage i holds this warp's positions of tile real0 + i
-    const int32_t* table = p.table + r * p.table_stride;
-    const T* kg = static_cast<const T*>(p.k) + g * p.k_s[1];
-    const T* vg = static_cast<const T*>(p.v) + g * p.v_s[1];
-    const int stages = real1 - real0;
-    const int first = real0 * S::kTile + warp * KEYS;  // the first position of stage 0
-    // Lane l copies row l % KEYS of a stage: the keys, the next KEYS lanes the
-    // values.
+  // ---- the ring: stage i holds this warp's positions of tile real0 + i
+    // The lanes hold the pages of the rows l % KEYS, and copy the 16-byte chunks
+    // 32 c + l of the keys and of the values.
     constexpr uint32_t ROWS_MASK = (1u << KEYS) - 1u;
-    const int my_row = lane % KEYS, side = lane / KEYS;
-    const T* const my_base = side == 0 ? kg : vg;
-    const int64_t page_step = side == 0 ? p.k_s[0] : p.v_s[0];
-    const int64_t row_step = side == 0 ? p.k_s[2] : p.v_s[2];
-    const uint32_t my_dst = side == 0 ? my_row * S::kPitchK : S::kHalf + my_row * S::kPitchV;
-    // The page of this lane's row in stage i and the row in it; nothing to read
-    // where the page is negative (past the length) or out of range.
-    struct Place {
-      int page, row;
+    constexpr int STEPS = KEYS * ROW / 32;
+    const int my_row = lane % KEYS;
+    // The page of position j of request q, wherever the table has one: whether
+    // the position counts is decided when its row is copied.
+    auto page_at = [&](int q, int j) -> int {
+      if (j >= p.max_keys) return -1;
+      return p.table[q * p.table_stride + fast_div(static_cast<uint32_t>(j), p.page)];
     };
-    auto place_of = [&](int i) -> Place {
-      const int j = first + i * S::kTile + my_row;
-      if (i >= stages || j >= n || j == fresh) return {INT_MIN, 0};
-      const int at = static_cast<int>(fast_div(static_cast<uint32_t>(j), p.page));
-      return {table[at], j - at * static_cast<int>(p.page.d)};
+    auto page_of = [&](int i) -> int {
+      return i < stages ? page_at(r, first + i * S::kTile + my_row) : -1;
     };
-    int filled = 0;
-    auto fill = [&](int i, const Place& place) {
-      if (i >= stages || failed) return;
-      const uint32_t stage = ring + put * S::kStage, bar = smem_u32(&s_bar[warp][put]);
-      const int j0 = first + i * S::kTile;
-      const int new_row = fresh - j0;  // the row of the new position, if 0 <= it < KEYS
-      const bool has_new = fresh >= 0 && new_row >= 0 && new_row < KEYS;
-      const bool in_range = static_cast<unsigned>(place.page) < static_cast<unsigned>(p.num_pages);
-      const uint32_t read = __ballot_sync(FULL, in_range) & ROWS_MASK;
-      const uint32_t live = read | (has_new ? 1u << new_row : 0u);
-      if (lane == 0) {
-        s_live[warp][put] = live;
-        tc::mbar_expect_tx(bar, 2 * __popc(read) * row_bytes);
+    int filled = 0;  // stages of the segment
+    auto fill = [&](int page) {  // the next stage, row l % KEYS from `page`
+      if (filled < stages) {
+        const uint32_t kd = ring + put * S::kStage, vd = kd + S::kHalf;
+        const int j0 = first + filled * S::kTile;
+        const int new_row = fresh - j0;  // the row of the new position, if 0 <= it < KEYS
+        const bool has_new = fresh >= 0 && new_row >= 0 && new_row < KEYS;
+        const bool exists = static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages);
+        const T* const kg = static_cast<const T*>(p.k) + g * p.k_s[1];
+        const T* const vg = static_cast<const T*>(p.v) + g * p.v_s[1];
+        if (aligned && j0 + KEYS <= n && !has_new && __all_sync(FULL, exists)) {
+          // one page and all of its rows: the chunks are a constant step apart
+          const int row0 = j0 - static_cast<int>(fast_div(static_cast<uint32_t>(j0), p.page) *
+                                                 p.page.d) + (ROW <= 32 ? lane / ROW : 0);
+          const int col = ROW <= 32 ? lane % ROW : lane;
+          const T* ks = kg + page * p.k_s[0] + row0 * p.k_s[2] + col * CH;
+          const T* vs = vg + page * p.v_s[0] + row0 * p.v_s[2] + col * CH;
+          const uint32_t kc = kd + (ROW <= 32 ? lane / ROW : 0) * S::kPitchK + col * 16;
+          const uint32_t vc = vd + (ROW <= 32 ? lane / ROW : 0) * S::kPitchV + col * 16;
+          if constexpr (ROW <= 32) {
+            const int64_t kn = (32 / ROW) * p.k_s[2], vn = (32 / ROW) * p.v_s[2];
+#pragma unroll
+            for (int c = 0; c < STEPS; ++c) {
+              copy_async(kc + c * (32 / ROW) * S::kPitchK, ks);
+              copy_async(vc + c * (32 / ROW) * S::kPitchV, vs);
+              ks += kn;
+              vs += vn;
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < STEPS; ++c) {
+              copy_async(kc + (c / 2) * S::kPitchK + (c % 2) * 512, ks + (c % 2) * 32 * CH);
+              copy_async(vc + (c / 2) * S::kPitchV + (c % 2) * 512, vs + (c % 2) * 32 * CH);
+              if (c % 2 == 1) {
+                ks += p.k_s[2];
+                vs += p.v_s[2];
+              }
+            }
+          }
+          if (lane == 0) s_live[warp][put] = ROWS_MASK;
+        } else {
+          // row by row: zeros for what does not count, nothing for the new row
+          const int j = j0 + my_row;
+          const bool counts = j < n && j != fresh;
+          if (counts && !exists) report(p.status, TVR_DEV_BAD_INDEX);
+          const uint32_t read = __ballot_sync(FULL, counts && exists) & ROWS_MASK;
+          if (lane == 0) s_live[warp][put] = read | (has_new ? 1u << new_row : 0u);
+          const int in_page =
+              j - static_cast<int>(fast_div(static_cast<uint32_t>(j), p.page) * p.page.d);
+          const int64_t ko = page * p.k_s[0] + in_page * p.k_s[2];
+          const int64_t vo = page * p.v_s[0] + in_page * p.v_s[2];
+#pragma unroll 1
+          for (int c = 0; c < STEPS; ++c) {
+            const int row = (c * 32 + lane) / ROW, col = (c * 32 + lane) % ROW;
+            const int64_t ks = __shfl_sync(FULL, ko, row), vs = __shfl_sync(FULL, vo, row);
+            const bool live = ((read >> row) & 1u) != 0 && col < cols;
+            if (has_new && row == new_row && col < cols) continue;
+            copy_async_or_zero(kd + row * S::kPitchK + col * 16, live ? kg + ks + col * CH : kg,
+                               live);
+            copy_async_or_zero(vd + row * S::kPitchV + col * 16, live ? vg + vs + col * CH : vg,
+                               live);
+          }
+        }
+        put = put + 1 == S::kStages ? 0 : put + 1;
+        ++filled;
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");  // a stage, or nothing
+    };
+    // The new position, if stage i (the one to be read) has it: from k_new and
+    // v_new into its row and its slot, while the stage's copies are under way.
+    auto place_new = [&](int i) {
+      const int row = fresh - (first + i * S::kTile);
+      if (fresh < 0 || row < 0 || row >= KEYS) return;
+      const uint32_t stage = ring + get * S::kStage;
+      const float* kn = p.k_new + r * p.kn_s[0] + g * p.kn_s[1];
+      const float* vn = p.v_new + r * p.vn_s[0] + g * p.vn_s[1];
+      const int64_t page = divide(slot, p.page.d), at = slot - page * p.page.d;
+      T* kc = static_cast<T*>(p.k) + page * p.k_s[0] + g * p.k_s[1] + at * p.k_s[2];
+      T* vc = static_cast<T*>(p.v) + page * p.v_s[0] + g * p.v_s[1] + at * p.v_s[2];
+      for (int col = lane; col < cols; col += 32) {
+        const uint4 kx = pack<T>(kn + col * CH), vx = pack<T>(vn + col * CH);
+        if (sub == 0) {
+          *reinterpret_cast<uint4*>(kc + col * CH) = kx;
+          *reinterpret_cast<uint4*>(vc + col * CH) = vx;
+        }
+        sts128(stage + row * S::kPitchK + col * 16, kx);
+        sts128(stage + S::kHalf + row * S::kPitchV + col * 16, vx);
+      }
+    };
+    // Waits for the stage to be read.
+    auto ready = [&]() {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
       __syncwarp();
-      if (in_range && side < 2) {
-        bulk_copy(stage + my_dst, my_base + place.page * page_step + place.row * row_step,
-                  row_bytes, bar);
-      }
-      if (has_new) {
-        const float* kn = p.k_new + r * p.kn_s[0] + g * p.kn_s[1];
-        const float* vn = p.v_new + r * p.vn_s[0] + g * p.vn_s[1];
-        const int64_t pg = slot / p.page.d, in = slot - pg * p.page.d;
-        T* kc = static_cast<T*>(p.k) + pg * p.k_s[0] + g * p.k_s[1] + in * p.k_s[2];
-        T* vc = static_cast<T*>(p.v) + pg * p.v_s[0] + g * p.v_s[1] + in * p.v_s[2];
-        for (int col = lane; col < cols; col += 32) {
-          const uint4 kx = pack<T>(kn + col * CH), vx = pack<T>(vn + col * CH);
-          if (sub == 0) {
-            *reinterpret_cast<uint4*>(kc + col * CH) = kx;
-            *reinterpret_cast<uint4*>(vc + col * CH) = vx;
-          }
-          sts128(stage + new_row * S::kPitchK + col * 16, kx);
-          sts128(stage + S::kHalf + new_row * S::kPitchV + col * 16, vx);
-        }
-      }
-      if (live != ROWS_MASK) {
-        if (!in_range && place.page != INT_MIN) report(p.status, TVR_DEV_BAD_INDEX);
-        for (uint32_t dead = ~live & ROWS_MASK; dead != 0; dead &= dead - 1) {
-          const uint32_t row = stage + S::kHalf + (__ffs(dead) - 1) * S::kPitchV;
-          for (int col = lane; col < cols; col += 32) {
-            sts128(row + col * 16, make_uint4(0, 0, 0, 0));
-          }
-        }
-      }
-      if (has_new || live != ROWS_MASK) fence_async();
-      put = put + 1 == S::kStages ? 0 : put + 1;
-      ++filled;
     };
-    // Waits for the stage to be read; false if it never comes.
-    auto ready = [&]() -> bool {
-      if (!tc::mbar_wait(smem_u32(&s_bar[warp][get]), parity, nullptr)) {
-        failed = true;
-        report(p.status, TVR_DEV_TIMEOUT_MMA);
-      }
-      failed = __any_sync(FULL, failed);
-      return !failed;
-    };
-    auto done = [&]() {
+    auto advance = [&]() {
       __syncwarp();
       get = get + 1 == S::kStages ? 0 : get + 1;
-      parity ^= get == 0 ? 1u : 0u;
     };
-    Place places[S::kStages];
+  // the first segment
+  slot = slot_of(r);
+  int ahead[EARLY + 1];  // pages of the stages to be filled next
 #pragma unroll
-    for (int i = 0; i < S::kStages; ++i) places[i] = place_of(i);
+  for (int i = 0; i <= EARLY; ++i) {
+    ahead[i] = page_at(r, max(0, t0 - kSetup) * S::kTile + warp * KEYS + i * S::kTile + my_row);
+  }
+  if (!begin()) return;
 #pragma unroll
-    for (int i = 0; i < S::kStages; ++i) fill(i, places[i]);
-    Place next = place_of(S::kStages);
+  for (int i = 0; i < EARLY; ++i) fill(ahead[i]);
+  int next_page = ahead[EARLY];
+
+  for (bool more = true; more;) {
+    if constexpr (MT > 0) {
+      const int page = next_page;
+      next_page = page_of(filled + 1);
+      fill(page);
+    }
+    const int h0 = g * p.group + sub * HEADS;
+    const int heads = min(HEADS, p.group - sub * HEADS);
+    // the segment after this one begins a unit, if there is one
+    const bool follow = u + (t1 - t0) < u_end;
+    const int n_unit = unit + 1 < units ? unit + 1 : 0, n_request = r + (unit + 1 < units ? 0 : 1);
+    if (follow) {
+#pragma unroll
+      for (int i = 0; i < EARLY; ++i) {
+        const int j = warp * KEYS + i * S::kTile + lane;
+        if (lane < KEYS && j < p.max_keys) {
+          fetch_async<4>(&s_pages[warp][i][lane],
+                         p.table + n_request * p.table_stride +
+                             fast_div(static_cast<uint32_t>(j), p.page));
+        }
+      }
+      if (lane == 0) {
+        fetch_async<4>(&s_length[warp], p.lens + n_request);
+        if (p.slots != nullptr) fetch_async<8>(&s_slot[warp], p.slots + n_request);
+      }
+    }
 
     if constexpr (MT == 0) {
-      constexpr int L = S::kLanes, NC = 16 / CH, STEP = 32 / L;
+      constexpr int L = DP / 16, NC = 16 / CH, STEP = 32 / L;
       const int lead = lane & (L - 1);
       // chunk c of this lane, in the order that it reads them
       const int turn = L < 8 ? (lane / L) & 1 : 0;
@@ -639,11 +718,9 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
         }
       }
       float m = -FLT_MAX, l = 0.f;  // m: one for the warp
-      for (int i = 0; i < stages && i < filled; ++i) {
-        if (!ready()) {  // what is in flight is still waited for
-          done();
-          continue;
-        }
+      for (int i = 0; i < stages; ++i) {
+        place_new(i);
+        ready();
         const uint32_t kd = ring + get * S::kStage, vd = kd + S::kHalf;
         const uint32_t live = s_live[warp][get];
 #pragma unroll
@@ -685,11 +762,10 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
             for (int e = 0; e < CH; ++e) o[c][e] = fmaf(w, v[e], o[c][e]);
           }
         }
-        done();
-        const int ahead = i + S::kStages;
-        const Place place = next;
-        next = place_of(ahead + 1);
-        fill(ahead, place);
+        advance();
+        const int page = next_page;
+        next_page = page_of(filled + 1);
+        fill(page);
       }
       // the rows' sums, lanes of even and odd rows apart as their orders differ
       constexpr int TURNED = L < 8 ? 2 * L : L;
@@ -720,7 +796,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
 #pragma unroll
-          for (int e = 0; e < CH; ++e) my_part[chunk(c) * CH + e] = o[c][e];
+          for (int e = 0; e < CH; ++e) part_of(warp)[chunk(c) * CH + e] = o[c][e];
         }
       }
       if (lane == 0) {
@@ -730,69 +806,73 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     } else {
       // lane = 4 grp + thr: rows grp and grp + 8 of a fragment (head grp's terms)
       constexpr int KS = S::kSteps, NT = KEYS / 8, MTR = MT > 0 ? MT : 1, XT = DP / 8;
-      constexpr float LIFT = S::kHalfs ? 7.f : 0.f;
+      constexpr float LIFT = HALFS ? 7.f : 0.f;
       const int grp = lane >> 2, thr = lane & 3;
-      const uint32_t query = smem_u32(smem + WARPS * S::kWarpRing) + lane * 16;
+      const uint32_t query0 = smem_u32(smem + WARPS * S::kWarpRing), query = query0 + lane * 16;
       const uint32_t third = query + MTR * KS * 512 - lane * 8;  // bf16: the third terms
 
       // ---- the query's fragments, shared by the warps
-      float unscale[MTR];  // f16: takes the scaling of head mt * 8 + grp back
-      if constexpr (S::kHalfs) {
-        for (int h = warp; h < HEADS; h += WARPS) {
+      // DP / 8 lanes a head, eight dimensions each
+      for (int x = tid; x < HEADS * (DP / 8); x += THREADS) {
+        const int h = x / (DP / 8), j = x % (DP / 8);
+        const float* src = p.q + r * p.q_s[0] + (h0 + h) * p.q_s[1] + 8 * j;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = h < heads && 8 * j + e < p.dim ? src[e] * p.scale_log2 : 0.f;
+        }
+        if constexpr (HALFS) {
           float top = 0.f;
-          const float* src = p.q + r * p.q_s[0] + (h0 + h) * p.q_s[1];
-          if (h < heads) {
-            for (int d = lane; d < p.dim; d += 32) top = fmaxf(top, fabsf(src[d] * p.scale_log2));
-          }
 #pragma unroll
-          for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+#pragma unroll
+          for (int d = 1; d < DP / 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
           // 2^(13 - exponent of top), within the range of fp32
-          const int e = static_cast<int>((__float_as_uint(top) >> 23) & 255u);
-          const int lift = e == 0 || e == 255 ? 0 : max(-100, min(100, 13 - (e - 127)));
-          if (lane == 0) s_top[h] = __uint_as_float(static_cast<uint32_t>(127 + lift) << 23);
-        }
-        __syncthreads();
-      }
-      for (int x = warp; x < MTR * KS; x += WARPS) {
-        const int mt = x / KS, ks = x - mt * KS, h = PACKED ? grp & 3 : mt * 8 + grp;
-        const float* src = p.q + r * p.q_s[0] + (h0 + h) * p.q_s[1];
-        const float sc = p.scale_log2 * (S::kHalfs ? s_top[h] : 1.f);
-        auto at = [&](int d) { return h < heads && d < p.dim ? src[d] * sc : 0.f; };
-        uint4 f;
-        if constexpr (sizeof(T) == 4) {
-          // step c * 2 + e takes, of chunk 4 c + thr, element 2 e as product
-          // thr and element 2 e + 1 as product thr + 4
-          const int d = (4 * (ks >> 1) + thr) * 4 + 2 * (ks & 1);
-          split_rounded(at(d), f.x, f.y);
-          split_rounded(at(d + 1), f.z, f.w);
-          sts128(query + x * 512, f);
-        } else {
-          const int d = 16 * ks + 2 * thr;
-          float a0 = at(d), a1 = at(d + 1), b0 = at(d + 8), b1 = at(d + 9);
-          f.x = take_term<T>(a0, a1);
-          f.z = take_term<T>(b0, b1);
-          f.y = take_term<T>(a0, a1);
-          f.w = take_term<T>(b0, b1);
-          if constexpr (PACKED) {
-            const uint32_t lo0 = take_term<T>(a0, a1), lo1 = take_term<T>(b0, b1);
-            if (grp >= 4) f = make_uint4(lo0, 0, lo1, 0);
-          }
-          sts128(query + x * 512, f);
-          if constexpr (S::kFrags == 2) {
-            const uint32_t lo0 = take_term<T>(a0, a1), lo1 = take_term<T>(b0, b1);
-            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(third + x * 256), "r"(lo0),
-                         "r"(lo1)
-                         : "memory");
-          }
-        }
-      }
-      if constexpr (S::kHalfs) {
+          const int e2 = static_cast<int>((__float_as_uint(top) >> 23) & 255u);
+          const int lift = e2 == 0 || e2 == 255 ? 0 : max(-100, min(100, 13 - (e2 - 127)));
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + lift) << 23);
 #pragma unroll
-        for (int mt = 0; mt < MTR; ++mt) {
-          unscale[mt] = __uint_as_float((254u << 23) - __float_as_uint(s_top[mt * 8 + grp]));
+          for (int e = 0; e < 8; ++e) v[e] *= up;
+          if (j == 0) s_top[h] = __uint_as_float(static_cast<uint32_t>(127 - lift) << 23);
+        }
+        const int mt = h / 8;
+        const uint32_t row = static_cast<uint32_t>(h % 8) * 4;  // its first lane
+        if constexpr (sizeof(T) == 4) {
+          // step 2 c + e takes, of chunk 4 c + thr, element 2 e as product thr
+          // and element 2 e + 1 as product thr + 4
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int chunk = 2 * j + (y >> 1), ks = 2 * (chunk >> 2) + (y & 1);
+            uint4 f;
+            split_rounded(v[2 * y], f.x, f.y);
+            split_rounded(v[2 * y + 1], f.z, f.w);
+            sts128(query0 + (mt * KS + ks) * 512 + (row + (chunk & 3)) * 16, f);
+          }
+        } else {
+          // step ks takes dimensions 16 ks + 2 thr and the next one as products
+          // 2 thr and 2 thr + 1, and those 8 further as 2 thr + 8 and 2 thr + 9
+          const int ks = mt * KS + (j >> 1);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t hi = take_term<T>(v[2 * y], v[2 * y + 1]);
+            const uint32_t mid = take_term<T>(v[2 * y], v[2 * y + 1]);
+            const uint32_t at = query0 + ks * 512 + (row + y) * 16 + (j & 1) * 8;
+            sts64(at, hi, mid);
+            if constexpr (PACKED) sts64(at + 256, take_term<T>(v[2 * y], v[2 * y + 1]), 0);
+            if constexpr (S::kFrags == 2) {
+              const uint32_t lo = take_term<T>(v[2 * y], v[2 * y + 1]);
+              asm volatile("st.shared.u32 [%0], %1;" ::"r"(query0 + MTR * KS * 512 + ks * 256 +
+                                                          (row + y) * 8 + (j & 1) * 4),
+                           "r"(lo)
+                           : "memory");
+            }
+          }
         }
       }
       __syncthreads();
+      float unscale[MTR];  // f16: takes the scaling of head mt * 8 + grp back
+#pragma unroll
+      for (int mt = 0; mt < MTR; ++mt) unscale[mt] = HALFS ? s_top[mt * 8 + grp] : 1.f;
 
       float o[MTR][XT][4], m[MTR], l[MTR];
 #pragma unroll
@@ -805,11 +885,9 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
           for (int e = 0; e < 4; ++e) o[mt][x][e] = 0.f;
         }
       }
-      for (int i = 0; i < stages && i < filled; ++i) {
-        if (!ready()) {  // what is in flight is still waited for
-          done();
-          continue;
-        }
+      for (int i = 0; i < stages; ++i) {
+        place_new(i);
+        ready();
         const uint32_t kd = ring + get * S::kStage, vd = kd + S::kHalf;
         const uint32_t live = s_live[warp][get];
 
@@ -885,7 +963,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
                 lo += s[mt][nt][1][e + 2];
               }
               float v = hi + lo;
-              if constexpr (S::kHalfs) v *= unscale[mt];
+              if constexpr (HALFS) v *= unscale[mt];
               if constexpr (PACKED) v += __shfl_xor_sync(FULL, v, 16);
               const bool in = ((live >> (nt * 8 + 2 * thr + e)) & 1u) != 0;
               z[mt][nt][e] = in ? v : -INFINITY;
@@ -1023,14 +1101,12 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
             }
           }
         }
-        done();
-        const int ahead = i + S::kStages;
-        const Place place = next;
-        next = place_of(ahead + 1);
-        fill(ahead, place);
+        advance();
+        const int page = next_page;
+        next_page = page_of(filled + 1);
+        fill(page);
       }
-      // the warp's part takes the place of its ring, which is drained: every
-      // copy into it has been waited for
+      // the ring is drained: every copy into it has been waited for
 #pragma unroll
       for (int mt = 0; mt < MTR; ++mt) {
         l[mt] += __shfl_xor_sync(FULL, l[mt], 1);
@@ -1040,7 +1116,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
           s_m[warp][mt * 8 + grp] = m[mt];
           s_l[warp][mt * 8 + grp] = l[mt];
         }
-        float* row = my_part + (mt * 8 + grp) * DP;
+        float* row = part_of(warp) + (mt * 8 + grp) * PART;
 #pragma unroll
         for (int x = 0; x < XT; ++x) {
           // the columns 2 thr and 2 thr + 1 of tile x
@@ -1051,10 +1127,41 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
             o1 += __shfl_xor_sync(FULL, o1, 16);
           }
           if (mine) {
-            row[d] = o0;
-            row[d + (sizeof(T) == 4 ? CH : 1)] = o1;
+            if constexpr (sizeof(T) == 4) {
+              row[d] = o0;
+              row[d + CH] = o1;
+            } else {
+              *reinterpret_cast<float2*>(row + d) = make_float2(o0, o1);
+            }
           }
         }
+      }
+    }
+
+    // ---- on to the next segment, whose copies are under way while the parts
+    // of this one are joined
+    const int d_r = r, d_count = count;
+    const bool whole = real0 == 0 && t1 == count, empty = n == 0;
+    const long long d_u = u, u_unit = u - t0;  // u_unit: the unit's first tile
+    constexpr int kPartStep = MT == 0 ? DP : S::kWarpRing / 4;  // floats between warps' parts
+    float* const parts = part_of(0);
+    more = follow;
+    if (follow) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      u += t1 - t0;
+      t0 = 0;
+      r = n_request;
+      unit = n_unit;
+      n = max(0, min(p.max_keys, s_length[warp]));
+      count = tiles(n);
+      slot = p.slots != nullptr ? s_slot[warp] : -1;
+      filled = 0;
+      more = begin();
+      if (more) {
+        next_page = page_of(EARLY);
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i) fill(s_pages[warp][i][my_row]);
       }
     }
 
@@ -1072,37 +1179,43 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
       }
       s_top[tid] = top;
       s_sum[tid] = sum;
+      s_inverse[tid] = 1.f / sum;
     }
     __syncthreads();
-    const bool whole = real0 == 0 && t1 == count;
-    const long long u_unit = u - t0;  // the unit's first tile
-    float* part = sp.parts + ((2 * cta + (u == u_first ? 0 : 1)) * HEADS) * S::kRecord;
-    for (int x = tid; x < heads * DP; x += THREADS) {
-      const int h = x / DP, d = x - h * DP;
-      float acc = 0.f;
+    float* const out = p.out + d_r * p.o_s[0] + h0 * p.o_s[1];
+    float* const lse =
+        p.lse != nullptr ? p.lse + static_cast<int64_t>(d_r) * p.heads + h0 : nullptr;
+    float* const part =
+        sp.parts + ((2 * cta + (d_u == u_first ? 0 : 1)) * HEADS) * S::kRecord;
+    for (int x = tid; x < heads * (DP / 4); x += THREADS) {
+      const int h = x / (DP / 4), d = 4 * (x % (DP / 4));
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) acc += parts0[w * kPartStep + x] * s_f[w][h];
-      if (whole) {
-        if (d < p.dim) {
-          p.out[r * p.o_s[0] + (h0 + h) * p.o_s[1] + d] = n > 0 ? acc / s_sum[h] : 0.f;
-        }
-      } else {
-        part[h * S::kRecord + d] = acc;
+      for (int w = 0; w < WARPS; ++w) {
+        const float4 o = *reinterpret_cast<const float4*>(parts + w * kPartStep + h * PART + d);
+        const float f = s_f[w][h];
+        acc.x = fmaf(o.x, f, acc.x);
+        acc.y = fmaf(o.y, f, acc.y);
+        acc.z = fmaf(o.z, f, acc.z);
+        acc.w = fmaf(o.w, f, acc.w);
+      }
+      if (!whole) {
+        *reinterpret_cast<float4*>(part + h * S::kRecord + d) = acc;
+      } else if (d < p.dim) {  // a whole number of fours
+        put_four(out + h * p.o_s[1] + d, acc, empty ? 0.f : s_inverse[h]);
       }
     }
     if (tid < heads) {
       if (!whole) {
         part[tid * S::kRecord + DP] = s_top[tid];
         part[tid * S::kRecord + DP + 1] = s_sum[tid];
-      } else if (p.lse != nullptr) {
-        p.lse[static_cast<int64_t>(r) * p.heads + h0 + tid] =
-            n > 0 ? s_top[tid] * 0.69314718055994531f + logf(s_sum[tid]) : -INFINITY;
+      } else if (lse != nullptr) {
+        lse[tid] = empty ? -INFINITY : s_top[tid] * 0.69314718055994531f + logf(s_sum[tid]);
       }
     }
     if (!whole) {
-      // CTAs of this unit: tile x belongs to CTA ((x + 1) ctas - 1) / total
-      const long long c0 = ((u_unit + kSetup + 1) * ctas - 1) / total;
-      const long long c1 = ((u_unit + count) * ctas - 1) / total;
+      const long long c0 = divide((u_unit + kSetup + 1) * ctas - 1, total);
+      const long long c1 = divide((u_unit + d_count) * ctas - 1, total);
       __threadfence();
       __syncthreads();
       if (tid == 0) s_last = atomicAdd(sp.counters + c0, 1) == static_cast<int>(c1 - c0) ? 1 : 0;
@@ -1110,40 +1223,38 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
       if (s_last != 0) {
         __threadfence();
         // c0's part is its first segment's only if the unit starts its range
-        const int late = c0 * total / ctas < u_unit ? 1 : 0;
+        const int late = divide(c0 * total, ctas) < u_unit ? 1 : 0;
         const int n_parts = static_cast<int>(c1 - c0) + 1;
         auto record = [&](int i, int h) -> const float* {
           const long long place = 2 * (c0 + i) + (i == 0 ? late : 0);
           return sp.parts + (place * HEADS + h) * S::kRecord;
         };
-        // factors [part][head] and, after them, the groups' sums: the ring is free
-        float* const s_join = reinterpret_cast<float*>(smem);
         for (int h = warp; h < heads; h += WARPS) {
           float top = -FLT_MAX, sum = 0.f;
           for (int i = lane; i < n_parts; i += 32) top = fmaxf(top, __ldcg(record(i, h) + DP));
 #pragma unroll
           for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
           for (int i = lane; i < n_parts; i += 32) {
-            const float f = exp2f(__ldcg(record(i, h) + DP) - top);
-            s_join[i * HEADS + h] = f;
-            sum += __ldcg(record(i, h) + DP + 1) * f;
+            sum += __ldcg(record(i, h) + DP + 1) * exp2f(__ldcg(record(i, h) + DP) - top);
           }
 #pragma unroll
           for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
           if (lane == 0) {
-            s_sum[h] = sum;
-            if (p.lse != nullptr) {
-              p.lse[static_cast<int64_t>(r) * p.heads + h0 + h] =
-                  top * 0.69314718055994531f + logf(sum);
-            }
+            s_top[h] = top;
+            s_inverse[h] = 1.f / sum;
+            if (lse != nullptr) lse[h] = top * 0.69314718055994531f + logf(sum);
           }
         }
         __syncthreads();
         // LANES lanes read a part's outputs, 16 bytes each and VECS of them;
-        // the GROUPS of lanes take the parts in turn
+        // the GROUPS of lanes take the parts in turn, and leave their sums where
+        // the warps' parts were
         constexpr int QUADS = HEADS * DP / 4, LANES = QUADS < 32 ? QUADS : 32;
         constexpr int VECS = QUADS / LANES, GROUPS = THREADS / LANES;
+        static_assert(GROUPS == WARPS || (MT == 0 && GROUPS * DP * 4 <= S::kPartBytes),
+                      "room for the groups' sums");
         const int group = tid / LANES, quad = tid % LANES;
+        auto sums_of = [&](int y) -> float* { return parts + y * kPartStep; };
         float acc[VECS][4];
 #pragma unroll
         for (int v = 0; v < VECS; ++v) acc[v][0] = acc[v][1] = acc[v][2] = acc[v][3] = 0.f;
@@ -1155,7 +1266,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
             const int x = (v * LANES + quad) * 4, h = x / DP;
             if (h < heads) {
               const float4 o = __ldcg(reinterpret_cast<const float4*>(rec + x + h * 4));
-              const float f = s_join[i * HEADS + h];
+              const float f = exp2f(__ldcg(rec + h * S::kRecord + DP) - s_top[h]);
               acc[v][0] = fmaf(o.x, f, acc[v][0]);
               acc[v][1] = fmaf(o.y, f, acc[v][1]);
               acc[v][2] = fmaf(o.z, f, acc[v][2]);
@@ -1163,37 +1274,29 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
             }
           }
         }
-        float* const s_group = s_join + ((n_parts * HEADS + 3) & ~3);
 #pragma unroll
         for (int v = 0; v < VECS; ++v) {
-          *reinterpret_cast<float4*>(s_group + group * HEADS * DP + (v * LANES + quad) * 4) =
+          *reinterpret_cast<float4*>(sums_of(group) + (v * LANES + quad) * 4) =
               make_float4(acc[v][0], acc[v][1], acc[v][2], acc[v][3]);
         }
         __syncthreads();
-        for (int x = tid; x < heads * DP; x += THREADS) {
-          const int h = x / DP, d = x - h * DP;
-          float sum = 0.f;
+        for (int x = tid; x < heads * (DP / 4); x += THREADS) {
+          const int h = x / (DP / 4), d = 4 * (x % (DP / 4));
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int y = 0; y < GROUPS; ++y) sum += s_group[y * HEADS * DP + x];
-          if (d < p.dim) p.out[r * p.o_s[0] + (h0 + h) * p.o_s[1] + d] = sum / s_sum[h];
+          for (int y = 0; y < GROUPS; ++y) {
+            const float4 o = *reinterpret_cast<const float4*>(sums_of(y) + h * DP + d);
+            sum.x += o.x;
+            sum.y += o.y;
+            sum.z += o.z;
+            sum.w += o.w;
+          }
+          if (d < p.dim) put_four(out + h * p.o_s[1] + d, sum, s_inverse[h]);
         }
         if (tid == 0) sp.counters[c0] = 0;
       }
     }
-    fence_async();
     __syncthreads();  // the shared parts are free for the next segment
-    zero_padding();
-
-    u += t1 - t0;
-    t0 = 0;
-    if (t1 == count && ++unit == units) {
-      unit = 0;
-      ++r;
-      if (r < sp.requests) {
-        n = length(r);
-        count = tiles(n);
-      }
-    }
   }
 }
 
