@@ -26,6 +26,9 @@ from dataclasses import dataclass, field
 
 import torch
 
+from . import paged
+from .paged import LogitRules, PagedCache
+
 
 @dataclass
 class GPT2Config:
@@ -289,6 +292,77 @@ def decode_step(model: GPT2, ids: torch.Tensor, cache: KVCache, pos: torch.Tenso
     nxt = F.linear(x, model.wte)[:, -1].argmax(-1, keepdim=True)
     torch.ops.tvarant.counter_add_(pos, 1)
     ids.copy_(nxt)
+    return ids
+
+
+def new_paged_cache(model: GPT2, requests: int, num_pages: int, page_size: int, max_len: int,
+                    device, dtype: torch.dtype = torch.float32) -> PagedCache:
+    """A paged cache of the model's layers and heads (``tvarant_b200.paged``)."""
+    cfg = model.cfg
+    return paged.new_paged_cache(cfg.n_layer, requests, num_pages, page_size, max_len, cfg.n_head,
+                                 cfg.n_head, cfg.d_model // cfg.n_head, device, dtype)
+
+
+def paged_prefill(model: GPT2, ids: torch.Tensor, cache: PagedCache, request: int) -> torch.Tensor:
+    """Takes the prompt ``ids`` [1, S] (int64, device) of a fresh request into
+    the cache and returns its logits [1, S, vocab], those of ``forward``.  The
+    other requests are as they were.  The pool must have the pages (the device
+    status word says if it had not)."""
+    F = torch.nn.functional
+    cfg = model.cfg
+    S, d, H = ids.shape[1], cfg.d_model, cfg.n_head
+    hd = d // H
+    scale = 1.0 / math.sqrt(hd)
+    new_lens = torch.zeros(cache.requests, dtype=torch.int32)
+    new_lens[request] = S
+    slots, positions, _ = cache.plan(new_lens.to(ids.device), tokens=S)
+    x = F.embedding(ids, model.wte) + F.embedding(positions.view(1, S), model.wpe)
+    for li, L in enumerate(model.layers):
+        h = F.layer_norm(x, (d,), L.ln1_g, L.ln1_b, 1e-5)
+        qkv = F.linear(h, L.w_qkv, L.b_qkv).view(S, 3, H, hd)
+        cache.append(li, qkv[:, 1], qkv[:, 2], slots)
+        q, k, v = qkv.permute(1, 2, 0, 3).unsqueeze(1)  # [1, H, S, hd] each
+        o = F.scaled_dot_product_attention(q, k, v, is_causal=True, scale=scale)
+        x = _linear_residual(x, o.transpose(1, 2).reshape(1, S, d), L.w_proj, L.b_proj)
+        h = F.layer_norm(x, (d,), L.ln2_g, L.ln2_b, 1e-5)
+        x = _linear_residual(x, _linear_silu(h, L.w_fc, L.b_fc), L.w_out, L.b_out)
+    return head(model, x)
+
+
+def paged_decode_step(model: GPT2, ids: torch.Tensor, cache: PagedCache, live: torch.Tensor,
+                      rules: LogitRules | None = None) -> torch.Tensor:
+    """One greedy decode step of every request r with ``live[r]`` = 1 (int32,
+    device; 0: idle, negative: the request ends and gives up its pages), for
+    the tvarant device.  ``ids`` [requests, 1] (int64, device) holds the
+    current tokens; each live request's is appended to its own pages and
+    attends to all of its positions.  ``rules`` adjust the logits before the
+    choice, and their histories take the chosen tokens.  Writes the next
+    tokens into ``ids`` and returns it (rows that are not live hold no token).
+    Nothing depends on host values, so the step can be captured once as a CUDA
+    graph (``tvarant_b200.graphs.Graph``) and replayed while requests come and
+    go."""
+    F = torch.nn.functional
+    cfg = model.cfg
+    R, d, H = ids.shape[0], cfg.d_model, cfg.n_head
+    hd = d // H
+    scale = 1.0 / math.sqrt(hd)
+    slots, positions, _ = cache.plan(live, tokens_per_request=1)
+    slots = slots.view(R)
+    x = F.embedding(ids, model.wte) + F.embedding(positions, model.wpe)
+    for li, L in enumerate(model.layers):
+        h = F.layer_norm(x, (d,), L.ln1_g, L.ln1_b, 1e-5)
+        qkv = F.linear(h, L.w_qkv, L.b_qkv).view(R, 3, H, hd)
+        o = cache.append_attend(li, qkv[:, 0], qkv[:, 1], qkv[:, 2], slots, scale)
+        x = _linear_residual(x, o.view(R, 1, d), L.w_proj, L.b_proj)
+        h = F.layer_norm(x, (d,), L.ln2_g, L.ln2_b, 1e-5)
+        x = _linear_residual(x, _linear_silu(h, L.w_fc, L.b_fc), L.w_out, L.b_out)
+    logits = head(model, x).view(R, cfg.vocab)
+    if rules is not None:
+        logits = rules.apply(logits)
+    nxt = logits.argmax(-1)
+    if rules is not None and rules.tokens is not None:
+        torch.ops.tvarant.history_append_(rules.tokens, rules.total_lens, nxt, live)
+    ids.copy_(nxt.view(R, 1))
     return ids
 
 
