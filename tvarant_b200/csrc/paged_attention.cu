@@ -1216,12 +1216,16 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     if (!whole) {
       const long long c0 = divide((u_unit + kSetup + 1) * ctas - 1, total);
       const long long c1 = divide((u_unit + d_count) * ctas - 1, total);
-      __threadfence();
+      // one thread's fence, after the barrier, orders the CTA's stores before
+      // the count, and the count before the CTA's loads
       __syncthreads();
-      if (tid == 0) s_last = atomicAdd(sp.counters + c0, 1) == static_cast<int>(c1 - c0) ? 1 : 0;
+      if (tid == 0) {
+        __threadfence();
+        s_last = atomicAdd(sp.counters + c0, 1) == static_cast<int>(c1 - c0) ? 1 : 0;
+        __threadfence();
+      }
       __syncthreads();
       if (s_last != 0) {
-        __threadfence();
         // c0's part is its first segment's only if the unit starts its range
         const int late = divide(c0 * total, ctas) < u_unit ? 1 : 0;
         const int n_parts = static_cast<int>(c1 - c0) + 1;
@@ -1229,21 +1233,40 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
           const long long place = 2 * (c0 + i) + (i == 0 ? late : 0);
           return sp.parts + (place * HEADS + h) * S::kRecord;
         };
-        for (int h = warp; h < heads; h += WARPS) {
-          float top = -FLT_MAX, sum = 0.f;
-          for (int i = lane; i < n_parts; i += 32) top = fmaxf(top, __ldcg(record(i, h) + DP));
-#pragma unroll
-          for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
-          for (int i = lane; i < n_parts; i += 32) {
-            sum += __ldcg(record(i, h) + DP + 1) * exp2f(__ldcg(record(i, h) + DP) - top);
+        // maximum and sum of each head over the parts: thread t takes head
+        // t % HEADS of every (THREADS / HEADS)th part
+        auto merge = [](float& top, float& sum, float m, float l) {
+          const float to = fmaxf(top, m);
+          sum = sum * exp2f(top - to) + l * exp2f(m - to);
+          top = to;
+        };
+        float top = -FLT_MAX, sum = 0.f;
+        if (tid % HEADS < heads) {
+#pragma unroll 4
+          for (int x = tid; x < n_parts * HEADS; x += THREADS) {
+            const float2 ml =
+                __ldcg(reinterpret_cast<const float2*>(record(x / HEADS, x % HEADS) + DP));
+            merge(top, sum, ml.x, ml.y);
           }
+        }
 #pragma unroll
-          for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
-          if (lane == 0) {
-            s_top[h] = top;
-            s_inverse[h] = 1.f / sum;
-            if (lse != nullptr) lse[h] = top * 0.69314718055994531f + logf(sum);
-          }
+        for (int x = HEADS; x < 32; x <<= 1) {
+          const float m = __shfl_xor_sync(FULL, top, x), l = __shfl_xor_sync(FULL, sum, x);
+          merge(top, sum, m, l);
+        }
+        if (lane < HEADS) {
+          s_m[warp][lane] = top;
+          s_l[warp][lane] = sum;
+        }
+        __syncthreads();
+        if (tid < heads) {
+          top = s_m[0][tid];
+          sum = s_l[0][tid];
+#pragma unroll
+          for (int w = 1; w < WARPS; ++w) merge(top, sum, s_m[w][tid], s_l[w][tid]);
+          s_top[tid] = top;
+          s_inverse[tid] = 1.f / sum;
+          if (lse != nullptr) lse[tid] = top * 0.69314718055994531f + logf(sum);
         }
         __syncthreads();
         // LANES lanes read a part's outputs, 16 bytes each and VECS of them;
