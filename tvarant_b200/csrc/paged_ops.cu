@@ -4,8 +4,10 @@
 
 #include "cluster.cuh"
 
+#include <algorithm>
 #include <climits>
 #include <cstring>
+#include <mutex>
 
 namespace tvr {
 namespace paged {
@@ -23,12 +25,15 @@ namespace {
 // Allocation j takes entry top - 1 - j, so every page and every token's slot
 // follows from the three prefix sums alone.
 //
-// One launch: every CTA of a cluster computes the prefix sums of all requests
-// in its shared memory (20 bytes a request), the cluster's threads share out
-// the new table entries, the tokens and the pages pushed; a search in a prefix
-// sum finds the request.  Nothing that a thread reads from memory is written
-// in the same call except the lengths and the count, which are written after a
-// cluster barrier that follows the sums: they may be updated in place.
+// One launch: every CTA computes the prefix sums of all requests in its shared
+// memory (20 bytes a request), the grid's threads share out the new table
+// entries, the pages pushed and the tokens; a search in a prefix sum finds the
+// request.  Nothing that a thread reads from memory is written in the same call
+// except, in place, the lengths and the count: then the grid is one cluster,
+// and they are written after a cluster barrier that follows the sums.
+// Bound by latencies: two rounds of loads, the sums and one search per output
+// (1000 requests, 41 thousand tokens: 19 us on a cluster of 8 CTAs of 1024
+// threads, 9 us on 148 of 256).
 constexpr int kMaxRequests = 8192;
 constexpr int kClusterCtas = 8;
 
@@ -82,18 +87,20 @@ __device__ __forceinline__ Sums shfl_up(const Sums& a, int d) {
           __shfl_up_sync(0xffffffffu, a.tokens, d)};
 }
 
-__global__ void __launch_bounds__(1024) page_plan_kernel(const __grid_constant__ PlanParams p) {
+// THREADS a CTA.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) page_plan_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ __align__(16) unsigned char plan_smem[];
   const int n = p.requests;
   long long* s_tokens = reinterpret_cast<long long*>(plan_smem);  // inclusive sums
   int* s_released = reinterpret_cast<int*>(s_tokens + n);
   int* s_need = s_released + n;
   int* s_seq = s_need + n;  // the length held; ~length for an ended request
-  __shared__ Sums s_warp[32];
+  constexpr int WARPS = THREADS / 32;
+  __shared__ Sums s_warp[WARPS];
   __shared__ int s_refused;
 
-  const int tid = threadIdx.x, threads = blockDim.x;
-  const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int free_count = max(0, min(p.num_pages, *p.count));
   auto pages_of = [&](long long positions) -> int {
     // positions < 2^31 + 2^31: a request that long is past any table
@@ -101,49 +108,64 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const __grid_constant__
     return static_cast<int>(fast_div(static_cast<uint32_t>(positions) + p.page.d - 1, p.page));
   };
 
-  // the prefix sums, blocks of `threads` consecutive requests after each other
-  Sums before = {0, 0, 0};
-  if (tid == 0) s_refused = 0;
-  for (int base = 0; base < n; base += threads) {
-    const int r = base + tid;
+  // the prefix sums: each thread takes consecutive requests, adds them up, and
+  // goes over them again with what lies before them
+  const int per_thread = (n + THREADS - 1) / THREADS;
+  const int r_begin = min(n, tid * per_thread), r_end = min(n, r_begin + per_thread);
+  auto request = [&](int r, int& held_seq) -> Sums {
     Sums own = {0, 0, 0};
-    int held_seq = 0;
-    if (r < n) {
-      const int seq = max(0, p.seq[r]), grow = p.grow[r];
-      const int held = pages_of(seq);
-      if (grow < 0) {
-        own.released = min(held, p.max_pages);
-        held_seq = ~seq;
-      } else {
-        const int want = pages_of(static_cast<long long>(seq) + grow);
-        const bool room = p.per_request == 0 || grow <= p.per_request;
-        own.need = room && want <= p.max_pages ? want - held : 0;
-        own.tokens = grow;
-        held_seq = seq;
-      }
+    const int seq = max(0, p.seq[r]), grow = p.grow[r];
+    const int held = pages_of(seq);
+    if (grow < 0) {
+      own.released = min(held, p.max_pages);
+      held_seq = ~seq;
+    } else {
+      const int want = pages_of(static_cast<long long>(seq) + grow);
+      const bool room = p.per_request == 0 || grow <= p.per_request;
+      own.need = room && want <= p.max_pages ? want - held : 0;
+      own.tokens = grow;
+      held_seq = seq;
     }
-    Sums sum = own;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const Sums below = shfl_up(sum, d);
-      if (lane >= d) sum = add(sum, below);
-    }
-    if (lane == 31) s_warp[warp] = sum;
-    __syncthreads();
-    Sums total = before;
-    for (int w = 0; w < warps; ++w) {
-      if (w == warp) sum = add(sum, total);
-      total = add(total, s_warp[w]);
-    }
-    if (r < n) {
-      s_released[r] = sum.released;
-      s_need[r] = sum.need;
-      s_tokens[r] = sum.tokens;
-      s_seq[r] = held_seq;
-    }
-    before = total;
-    __syncthreads();  // s_warp is free again, the sums are visible
+    return own;
+  };
+  if (tid == 0) s_refused = 0;
+  Sums mine = {0, 0, 0};
+  for (int r = r_begin; r < r_end; ++r) {
+    int held_seq;
+    mine = add(mine, request(r, held_seq));
   }
+  Sums sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const Sums below = shfl_up(sum, d);
+    if (lane >= d) sum = add(sum, below);
+  }
+  if (lane == 31) s_warp[warp] = sum;
+  __syncthreads();
+  if (warp == 0 && lane < WARPS) {
+    constexpr unsigned LANES = WARPS == 32 ? 0xffffffffu : (1u << (WARPS & 31)) - 1u;
+    Sums w = s_warp[lane];
+#pragma unroll
+    for (int d = 1; d < WARPS; d <<= 1) {
+      const Sums below = {__shfl_up_sync(LANES, w.released, d), __shfl_up_sync(LANES, w.need, d),
+                          __shfl_up_sync(LANES, w.tokens, d)};
+      if (lane >= d) w = add(w, below);
+    }
+    s_warp[lane] = w;
+  }
+  __syncthreads();
+  const Sums before = s_warp[WARPS - 1];  // of all requests
+  if (warp > 0) sum = add(sum, s_warp[warp - 1]);
+  sum = {sum.released - mine.released, sum.need - mine.need, sum.tokens - mine.tokens};
+  for (int r = r_begin; r < r_end; ++r) {
+    int held_seq;
+    sum = add(sum, request(r, held_seq));
+    s_released[r] = sum.released;
+    s_need[r] = sum.need;
+    s_tokens[r] = sum.tokens;
+    s_seq[r] = held_seq;
+  }
+  __syncthreads();
   const int top = free_count + before.released;
   // Admitted: a request that fits its table row and the token arrays, and
   // needs no page or ends within the stack.  The sums count every request that
@@ -167,14 +189,14 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const __grid_constant__
     return p.table[q * p.table_stride + at];
   };
   // pages taken: the needs are taken in order until one does not fit
-  int cut = first_above(s_need, n, top);
-  if (p.per_request == 0) {
+  int cut = before.need <= top ? n : first_above(s_need, n, top);
+  if (p.per_request == 0 && before.tokens > p.tokens) {
     cut = min(cut, first_above(s_tokens, n, static_cast<long long>(p.tokens)));
   }
   const int taken = cut > 0 ? s_need[cut - 1] : 0;
 
-  const int64_t step = static_cast<int64_t>(gridDim.x) * threads;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * threads + tid;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * THREADS;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * THREADS + tid;
   for (int64_t j = first; j < taken; j += step) {
     const int r = first_above(s_need, n, static_cast<int>(j));
     const int at = pages_of(s_seq[r]) + static_cast<int>(j) - (r > 0 ? s_need[r - 1] : 0);
@@ -215,9 +237,9 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const __grid_constant__
     if (p.rows != nullptr) p.rows[t] = live ? r : -1;
   }
 
-  cluster_sync();  // every CTA has read the lengths and the count
+  cluster_sync();  // in place: every CTA has read the lengths and the count
   if (blockIdx.x == 0) {
-    for (int r = tid; r < n; r += threads) {
+    for (int r = tid; r < n; r += THREADS) {
       const int seq = s_seq[r];
       const int grow = static_cast<int>(s_tokens[r] - (r > 0 ? s_tokens[r - 1] : 0));
       const bool in = admitted(r);
@@ -228,6 +250,33 @@ __global__ void __launch_bounds__(1024) page_plan_kernel(const __grid_constant__
     __syncthreads();
     if (tid == 0 && s_refused != 0) report(p.status, TVR_DEV_CACHE_FULL);
   }
+}
+
+template <int THREADS>
+int launch_plan(const PlanParams& p, unsigned ctas, unsigned cluster, cudaStream_t stream) {
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  const int dev = current_device();
+  std::call_once(once[dev & 63], [&]() {
+    attr_err[dev & 63] =
+        cudaFuncSetAttribute(page_plan_kernel<THREADS>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRequests * 20);
+  });
+  TVR_CUDA_TRY(attr_err[dev & 63]);
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.requests) * 20;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  TVR_CUDA_TRY(cudaLaunchKernelEx(&cfg, page_plan_kernel<THREADS>, p));
+  return TVR_OK;
 }
 
 // ---- append -------------------------------------------------------------------
@@ -397,26 +446,13 @@ extern "C" int tvr_page_plan(const tvr_page_pool* pool, const int32_t* seq_lens,
   p.tokens = tokens;
   p.per_request = tokens_per_request;
   p.status = device_status_ptr(dev);
-  const size_t smem = static_cast<size_t>(p.requests) * 20;
-  if (smem > 47 * 1024) {
-    TVR_CUDA_TRY(cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kMaxRequests * 20));
-  }
-  const int threads = 1024;
-  cudaLaunchAttribute attr[1] = {};
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kClusterCtas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kClusterCtas);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = as_stream(stream);
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  TVR_CUDA_TRY(cudaLaunchKernelEx(&cfg, page_plan_kernel, p));
-  return TVR_OK;
+  // In place: one CTA, or one cluster where there are more tokens than a few a
+  // thread.  Otherwise a CTA for each 256 tokens, up to one an SM.
+  const bool in_place = seq_lens_out == seq_lens || free_count_out == free_count;
+  if (tokens <= 4 * 256) return launch_plan<256>(p, 1, 1, as_stream(stream));
+  if (in_place) return launch_plan<1024>(p, kClusterCtas, kClusterCtas, as_stream(stream));
+  const int64_t ctas = std::min<int64_t>(sm_count(dev), ceil_div(tokens, 256));
+  return launch_plan<256>(p, static_cast<unsigned>(ctas), 1, as_stream(stream));
 }
 
 extern "C" int tvr_paged_append(const tvr_paged_kv* cache, const float* k_new, const float* v_new,
