@@ -230,13 +230,20 @@ struct Stream {
   // MT = 0: the warps' parts, or the sums of eight groups of lanes that join a
   // unit's parts; MT > 0: in the ring
   static constexpr int kPartBytes = MT == 0 ? (DP == 64 ? 8 : 4) * DP * 4 : 0;
-  // as many stages as an SM's shared memory holds, four at most
-  static constexpr int kRoom = 225 * 1024 / kCtasPerSm - (MT == 2 ? 1792 : 1024) - kQueryBytes -
-                               kPartBytes;
-  static constexpr int kStages =
-      kRoom / (kWarps * kStage) < 4 ? kRoom / (kWarps * kStage) : 4;
+  // As many stages as an SM's shared memory (228 KB, one of it taken by each
+  // CTA) holds, four at most; besides the ring there are the arrays declared in
+  // the kernel.
+  static constexpr int dynamic_bytes(int stages) {
+    return kWarps * stages * kStage + kQueryBytes + kPartBytes;
+  }
+  static constexpr bool fits(int stages) {
+    const int arrays = 128 + kWarps * (4 * stages + 12 * kHeads + 16) + 12 * kHeads +
+                       4 * kWarps * (MT == 0 ? stages : stages - 1) * kKeys;
+    return dynamic_bytes(stages) + arrays <= 228 * 1024 / kCtasPerSm - 1024;
+  }
+  static constexpr int kStages = fits(4) ? 4 : fits(3) ? 3 : fits(2) ? 2 : 1;
   static constexpr int kWarpRing = kStages * kStage;
-  static constexpr int kSmem = kWarps * kWarpRing + kQueryBytes + kPartBytes;
+  static constexpr int kSmem = dynamic_bytes(kStages);
   static_assert(kStages >= 2 && kKeys <= 16, "the ring");
   static_assert(MT == 0 || kStage >= kHeads * (DP + 8) * 4, "a part takes the place of a stage");
   static constexpr int kRecord = DP + 4;  // floats of one head's part: output, maximum, sum
