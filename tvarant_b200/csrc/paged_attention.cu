@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long s_scan[WARPS];
   __shared__ long long s_before;
-  __shared__ int s_request, s_last;
+  __shared__ int s_request, s_found, s_last;
   __shared__ uint32_t s_live[WARPS][S::kStages];
   __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_f[WARPS][HEADS];
   __shared__ float s_top[HEADS], s_sum[HEADS], s_inverse[HEADS];
@@ -460,7 +460,8 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     for (int w = 0; w < WARPS - 1; ++w) x += w < warp ? s_scan[w] : 0;
     return x;
   };
-  const int my_tiles = tid < sp.requests ? tiles(length(tid)) : 0;
+  const int my_length = tid < sp.requests ? length(tid) : 0;
+  const int my_tiles = tid < sp.requests ? tiles(my_length) : 0;
   const long long my_end = scan(my_tiles);
   long long head_tiles = 0, total = 0;
 #pragma unroll
@@ -489,16 +490,19 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     const long long target = divide(u, units);
     if (my_tiles > 0 && my_end > target && my_end - my_tiles <= target) {
       s_request = tid;
+      s_found = my_length;
       s_before = my_end - my_tiles;
     }
     long long before = head_tiles;
     for (int base = THREADS; before <= target; base += THREADS) {
       __syncthreads();
       const int q = base + tid;
-      const int t = q < sp.requests ? tiles(length(q)) : 0;
+      const int of_q = q < sp.requests ? length(q) : 0;
+      const int t = q < sp.requests ? tiles(of_q) : 0;
       const long long end = before + scan(t);
       if (q < sp.requests && end > target && end - t <= target) {
         s_request = q;
+        s_found = of_q;
         s_before = end - t;
       }
 #pragma unroll
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     }
     __syncthreads();
     r = s_request;
-    n = length(r);
+    n = s_found;
   }
   int count = tiles(n);
   const long long in_request = u - s_before * units;
