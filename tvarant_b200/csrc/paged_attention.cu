@@ -190,7 +190,8 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
 // A lane's scores are its own weights of the second product, and rows h and
 // h + 8 of a sum are in one lane: nothing is exchanged between lanes.
 constexpr int kMaxCtas = 640;  // bound on a launch's CTAs; sizes the workspace
-constexpr int kCounterBytes = 4096;
+constexpr int kCounterBytes = 8192;  // three counters a CTA
+constexpr int kJoinAtOnce = 24, kJoinGroup = 16;
 constexpr float kSlack = 8.f;
 constexpr int kSetup = 3;
 
@@ -221,6 +222,8 @@ struct Stream {
   static constexpr int kHalf = kKeys * kPitchK;  // keys, then values
   static constexpr int kStage = kHalf + kKeys * kPitchV;
   static constexpr int kTile = kWarps * kKeys;
+  // the least that a CTA takes: parts of more heads are more to join
+  static constexpr int kShare = MT == 0 ? 2 : 4;
   static constexpr int kHeads = MT == 0 ? 1 : PACKED ? 4 : 8 * MT;
   static_assert(!PACKED || (kBf16 && MT == 1), "packed rows");
   // query fragments of a k step of 16 (f32: 8): 16 bytes a lane, for bf16 8 more
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     for (int w = 0; w < WARPS; ++w) total += s_scan[w];
   }
   total *= units;
-  const long long ctas = min(static_cast<long long>(gridDim.x), total);
+  const long long ctas = min(static_cast<long long>(gridDim.x), max(1ll, total / S::kShare));
   const long long cta = blockIdx.x;
   if (cta >= ctas) return;
   // tile x belongs to CTA ((x + 1) ctas - 1) / total; CTA c begins at c total / ctas
@@ -484,7 +487,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     return ((x | y) >> 32) == 0 ? static_cast<uint32_t>(x) / static_cast<uint32_t>(y) : x / y;
   };
   long long u = divide(cta * total, ctas);
-  const long long u_first = u, u_end = divide((cta + 1) * total, ctas);
+  const long long u_end = divide((cta + 1) * total, ctas);
   int r, n;
   {
     const long long target = divide(u, units);
@@ -1153,7 +1156,8 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     // of this one are joined
     const int d_r = r, d_count = count;
     const bool whole = real0 == 0 && t1 == count, empty = n == 0;
-    const long long d_u = u, u_unit = u - t0;  // u_unit: the unit's first tile
+    const int real_from = real0;
+    const long long u_unit = u - t0;  // the unit's first tile
     constexpr int kPartStep = MT == 0 ? DP : S::kWarpRing / 4;  // floats between warps' parts
     float* const parts = part_of(0);
     more = follow;
@@ -1197,7 +1201,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     float* const lse =
         p.lse != nullptr ? p.lse + static_cast<int64_t>(d_r) * p.heads + h0 : nullptr;
     float* const part =
-        sp.parts + ((2 * cta + (d_u == u_first ? 0 : 1)) * HEADS) * S::kRecord;
+        sp.parts + ((2 * cta + (real_from == 0 ? 1 : 0)) * HEADS) * S::kRecord;
     for (int x = tid; x < heads * (DP / 4); x += THREADS) {
       const int h = x / (DP / 4), d = 4 * (x % (DP / 4));
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1227,25 +1231,30 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     if (!whole) {
       const long long c0 = divide((u_unit + kSetup + 1) * ctas - 1, total);
       const long long c1 = divide((u_unit + d_count) * ctas - 1, total);
-      // one thread's fence, after the barrier, orders the CTA's stores before
-      // the count, and the count before the CTA's loads
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();
-        s_last = atomicAdd(sp.counters + c0, 1) == static_cast<int>(c1 - c0) ? 1 : 0;
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last != 0) {
-        // c0's part is its first segment's only if the unit starts its range
-        const int late = divide(c0 * total, ctas) < u_unit ? 1 : 0;
-        const int n_parts = static_cast<int>(c1 - c0) + 1;
-        auto record = [&](int i, int h) -> const float* {
-          const long long place = 2 * (c0 + i) + (i == 0 ? late : 0);
-          return sp.parts + (place * HEADS + h) * S::kRecord;
-        };
-        // maximum and sum of each head over the parts: thread t takes head
-        // t % HEADS of every (THREADS / HEADS)th part
+      const int n_parts = static_cast<int>(c1 - c0) + 1;
+      // part i of the unit: of CTA c0 its last segment, of the others their first
+      auto record = [&](int i) -> float* {
+        return sp.parts + ((2 * (c0 + i) + (i == 0 ? 1 : 0)) * HEADS) * S::kRecord;
+      };
+      // Whether this CTA is the last of `arrivals`.  One thread's fence, after
+      // the barrier, orders the CTA's stores before the count, and the count
+      // before the CTA's loads.
+      auto last_of = [&](int* counter, int arrivals) -> bool {
+        __syncthreads();
+        if (tid == 0) {
+          __threadfence();
+          s_last = atomicAdd(counter, 1) == arrivals - 1 ? 1 : 0;
+          __threadfence();
+          if (s_last != 0) *counter = 0;  // nobody else arrives
+        }
+        __syncthreads();
+        return s_last != 0;
+      };
+      // Joins `count` parts from part `from` on, every `every`th: into the
+      // outputs, or into the first of them.
+      auto join = [&](int from, int every, int count, bool into_outputs) {
+        // maximum and sum of each head: thread t takes head t % HEADS of every
+        // (THREADS / HEADS)th part
         auto merge = [](float& top, float& sum, float m, float l) {
           const float to = fmaxf(top, m);
           sum = sum * exp2f(top - to) + l * exp2f(m - to);
@@ -1254,9 +1263,9 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
         float top = -FLT_MAX, sum = 0.f;
         if (tid % HEADS < heads) {
 #pragma unroll 4
-          for (int x = tid; x < n_parts * HEADS; x += THREADS) {
-            const float2 ml =
-                __ldcg(reinterpret_cast<const float2*>(record(x / HEADS, x % HEADS) + DP));
+          for (int x = tid; x < count * HEADS; x += THREADS) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(
+                record(from + x / HEADS * every) + x % HEADS * S::kRecord + DP));
             merge(top, sum, ml.x, ml.y);
           }
         }
@@ -1276,8 +1285,9 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
 #pragma unroll
           for (int w = 1; w < WARPS; ++w) merge(top, sum, s_m[w][tid], s_l[w][tid]);
           s_top[tid] = top;
+          s_sum[tid] = sum;
           s_inverse[tid] = 1.f / sum;
-          if (lse != nullptr) lse[tid] = top * 0.69314718055994531f + logf(sum);
+          if (into_outputs && lse != nullptr) lse[tid] = top * 0.69314718055994531f + logf(sum);
         }
         __syncthreads();
         // LANES lanes read a part's outputs, 16 bytes each and VECS of them;
@@ -1293,8 +1303,8 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
 #pragma unroll
         for (int v = 0; v < VECS; ++v) acc[v][0] = acc[v][1] = acc[v][2] = acc[v][3] = 0.f;
 #pragma unroll 2
-        for (int i = group; i < n_parts; i += GROUPS) {
-          const float* rec = record(i, 0);
+        for (int i = group; i < count; i += GROUPS) {
+          const float* rec = record(from + i * every);
 #pragma unroll
           for (int v = 0; v < VECS; ++v) {
             const int x = (v * LANES + quad) * 4, h = x / DP;
@@ -1314,20 +1324,45 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
               make_float4(acc[v][0], acc[v][1], acc[v][2], acc[v][3]);
         }
         __syncthreads();
+        float* const into = record(from);
         for (int x = tid; x < heads * (DP / 4); x += THREADS) {
           const int h = x / (DP / 4), d = 4 * (x % (DP / 4));
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          float4 sums = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int y = 0; y < GROUPS; ++y) {
             const float4 o = *reinterpret_cast<const float4*>(sums_of(y) + h * DP + d);
-            sum.x += o.x;
-            sum.y += o.y;
-            sum.z += o.z;
-            sum.w += o.w;
+            sums.x += o.x;
+            sums.y += o.y;
+            sums.z += o.z;
+            sums.w += o.w;
           }
-          if (d < p.dim) put_four(out + h * p.o_s[1] + d, sum, s_inverse[h]);
+          if (!into_outputs) {
+            *reinterpret_cast<float4*>(into + h * S::kRecord + d) = sums;
+          } else if (d < p.dim) {
+            put_four(out + h * p.o_s[1] + d, sums, s_inverse[h]);
+          }
         }
-        if (tid == 0) sp.counters[c0] = 0;
+        if (!into_outputs && tid < heads) {
+          *reinterpret_cast<float2*>(into + tid * S::kRecord + DP) =
+              make_float2(s_top[tid], s_sum[tid]);
+        }
+      };
+      if (n_parts <= kJoinAtOnce) {
+        if (last_of(sp.counters + c0, n_parts)) join(0, 1, n_parts, true);
+      } else {
+        // many parts: the last CTA of each kJoinGroup joins theirs, the last of
+        // these what they made of them
+        const int mine = static_cast<int>(cta - c0), begin_at = mine / kJoinGroup * kJoinGroup;
+        const int members = min(kJoinGroup, n_parts - begin_at);
+        const int groups = (n_parts + kJoinGroup - 1) / kJoinGroup;
+        // counters of the first group and of a later one, which may begin with
+        // the last part of this unit where the next unit's first group does
+        int* const counter =
+            sp.counters + (begin_at == 0 ? kMaxCtas + c0 : 2 * kMaxCtas + c0 + begin_at);
+        if (last_of(counter, members)) {
+          join(begin_at, 1, members, false);
+          if (last_of(sp.counters + c0, groups)) join(0, kJoinGroup, groups, true);
+        }
       }
     }
     __syncthreads();  // the shared parts are free for the next segment
