@@ -155,6 +155,24 @@ def test_parts_alone(lib, parts):
         assert np.array_equal(got, d["x"])
 
 
+@pytest.mark.parametrize("history", [32767, 32768, 40000])
+@pytest.mark.parametrize("vocab", [5003, 70001])
+def test_counters_of_both_widths(lib, vocab, history):
+    """A token that makes up the whole history, with or without a prompt before
+    it, and others beside it: the counts of neighbours stay apart."""
+    d = _make(np.random.default_rng(history), 3, vocab, history, 5, 3)
+    d["total"][:] = history
+    d["tokens"][0] = 4000
+    d["tokens"][1] = 4001
+    d["tokens"][1, ::2] = 4000
+    d["tokens"][2, :9000] = 4097
+    d["prompt"][:] = [0, 5, 0]
+    d["freq"][:] = [0.001, -0.002, 0.5]
+    got = _run(lib, d, ALL)
+    want, bound = _want(d, ALL)
+    _check(got, want, bound)
+
+
 def test_in_place_and_with_strides(lib):
     import torch
 
