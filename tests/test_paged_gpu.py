@@ -436,6 +436,22 @@ def test_attention_split_over_many_ctas(lib, heads, kv_heads, lens, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("heads, kv_heads, lens", [
+    (16, 1, LENS * 4 + [33, 400, 70]), (16, 1, LENS * 4 + [33, 400, 70, 9]),
+    (9, 1, [130] * 63 + [9000]), (40, 2, LENS * 3), (24, 1, [5] * 65),
+])
+def test_attention_of_more_heads_than_a_block_of_rows(lib, heads, kv_heads, lens, dim, dtype):
+    """Units of 8 and of 16 heads, whole and with heads to spare, on both sides of
+    64 (request, key head) pairs."""
+    c = Case(lib, lens, heads, kv_heads, dim, 16, dtype, seed=dim)
+    out, lse = c.check(append=True)
+    again, lse2 = c.run(append=True)
+    assert np.array_equal(out, again) and np.array_equal(lse, lse2)
+    assert _status(lib) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads, kv_heads", [(3, 3), (8, 2)])
 def test_append_form_is_append_then_attend(lib, heads, kv_heads, dtype):
     import torch
