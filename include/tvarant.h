@@ -393,10 +393,13 @@ int tvr_paged_append(const tvr_paged_kv* cache, const float* k_new, const float*
  * to the pages' type) and written to slots[r], which has to be that
  * position's slot: the same as tvr_paged_append and then this call.
  * A page id or slot out of range is dropped (the position does not count)
- * and sets TVR_DEV_BAD_INDEX.  head_dim is at most 256 (TVR_ERR_UNSUPPORTED
- * above).  `workspace` is device memory of tvr_paged_attention_workspace
- * bytes, zeroed before its first use, that no two calls use at the same time;
- * each call leaves it ready for the next. */
+ * and sets TVR_DEV_BAD_INDEX.  What pages hold at positions that do not
+ * count is not used.  Keys and values at positions that count are finite: an
+ * infinite or NaN one may make its request's outputs NaN where the formula
+ * has a value, and reaches no other request.  head_dim is at most 256
+ * (TVR_ERR_UNSUPPORTED above).  `workspace` is device memory of
+ * tvr_paged_attention_workspace bytes, zeroed before its first use, that no
+ * two calls use at the same time; each call leaves it ready for the next. */
 int tvr_paged_attention(const tvr_paged_kv* cache, const float* q, const float* k_new,
                         const float* v_new, const int64_t* slots, const int32_t* block_table,
                         int64_t table_stride, int64_t max_pages, const int32_t* seq_lens,
