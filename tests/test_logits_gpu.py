@@ -173,6 +173,30 @@ def test_counters_of_both_widths(lib, vocab, history):
     _check(got, want, bound)
 
 
+@pytest.mark.parametrize("bits", [32, 64])
+@pytest.mark.parametrize("rows, vocab, history, biases, masks", [
+    (700, 2053, 90, 10, 600), (900, 33, 5, 40, 3), (320, 4099, 700, 300, 320), (160, 40001, 300, 20, 7),
+    (601, 9000, 0, 3, 0),
+])
+def test_many_rows(lib, rows, vocab, history, biases, masks, bits):
+    """Rows enough for many CTAs an SM, also in place and with rows that start
+    anywhere; the same bits every time."""
+    import torch
+
+    d = _make(np.random.default_rng(rows), rows, vocab, max(1, history), biases, max(1, masks), bits)
+    parts = [x for x in ALL if (history or x not in ("tokens", "prompt")) and
+             (masks or x not in ("masks", "mask_rows"))]
+    want, bound = _want(d, parts)
+    got = _run(lib, d, parts)
+    _check(got, want, bound)
+    assert np.array_equal(got, _run(lib, d, parts), equal_nan=True)
+    buf = torch.full((rows, vocab + 10), math.nan, device="cuda")
+    x = buf[:, 3:3 + vocab]
+    x.copy_(torch.from_numpy(d["x"]))
+    _check(_run(lib, d, parts, x=x, out=x), want, bound)
+    assert torch.isnan(buf[:, :3]).all() and torch.isnan(buf[:, 3 + vocab:]).all()
+
+
 def test_in_place_and_with_strides(lib):
     import torch
 
