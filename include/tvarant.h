@@ -557,6 +557,16 @@ int tvr_history_append(void* tokens, int token_bits, int64_t tokens_stride, int3
                        const int64_t* ids, const int32_t* live, int64_t rows, int64_t capacity,
                        void* stream);
 
+/* The end of a decode step: for every row whose token the step has taken into
+ * the cache, slots[r] >= 0 as tvr_page_plan wrote it, current[r] = next[r], and
+ * next[r] joins the row's history as in tvr_history_append (tokens and lens
+ * NULL: no histories).  Rows that are idle or ended, or that the plan refused,
+ * keep their token and history, so that a refused token can be tried again.
+ * No reference counterpart. */
+int tvr_advance_tokens(int64_t* current, const int64_t* next, const int64_t* slots, void* tokens,
+                       int token_bits, int64_t tokens_stride, int32_t* lens, int64_t rows,
+                       int64_t capacity, void* stream);
+
 /* Triangular mask of dense [batch, rows, cols]: out = x where
  * col - row >= diagonal (upper != 0, triu) or col - row <= diagonal (tril),
  * else 0.  elem_size 1, 4 or 8.  No reference kernel (CPU fallback there). */

@@ -172,6 +172,7 @@ SIGNATURES: dict[str, list] = {
                             _vp, _vp, _i64, _i64, _pi64, _f32, _vp, _i64, _vp],
     "tvr_paged_attention_workspace": [_i64, _i64, _i64, _pi64],
     "tvr_history_append": [_vp, _i32, _i64, _vp, _vp, _vp, _i64, _i64, _vp],
+    "tvr_advance_tokens": [_vp, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _i64, _vp],
     "tvr_adjust_logits": [_vp, _i64, _vp, _i64, _i64, _i64, ctypes.POINTER(LogitRules), _vp],
     "tvr_attention_fwd": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _pi64, _pi64,
                           _pi64, _pi64, _f32, _i32, _i32, _vp],

@@ -1,8 +1,8 @@
 // The paged KV cache of many requests on the tvarant device: tvarant::page_plan
 // (block tables and slot maps), paged_append_, paged_attention and
-// paged_attention_append, and tvarant::adjust_logits with
-// history_append_ for the choice of the next token.  The reference has none
-// of them.
+// paged_attention_append, and tvarant::adjust_logits with history_append_ and
+// advance_tokens_ for the choice of the next token.  The reference has none of
+// them.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/library.h>
@@ -308,6 +308,36 @@ void history_append_(at::Tensor& tokens, at::Tensor& lens, const at::Tensor& ids
                              tokens.size(1), current_stream_handle()));
 }
 
+// current[r] = next[r] for the rows with slots[r] >= 0, whose histories (tokens
+// and lens, both or none) take next[r] too (tvr_advance_tokens).
+void advance_tokens_(at::Tensor& current, const at::Tensor& next, const at::Tensor& slots,
+                     std::optional<at::Tensor> tokens, std::optional<at::Tensor> lens) {
+  constexpr const char* op = "advance_tokens_";
+  TORCH_CHECK(is_device(current), op, ": expected tvarant tensors");
+  const int64_t rows = current.numel();
+  check_vector(current, rows, at::kLong, current, op, "current");
+  check_vector(next, rows, at::kLong, current, op, "next");
+  check_vector(slots, rows, at::kLong, current, op, "slots");
+  const bool some = tokens.has_value() && tokens->defined();
+  TORCH_CHECK(some == (lens.has_value() && lens->defined()), op, ": tokens and lens come together");
+  if (some) {
+    TORCH_CHECK(tokens->device() == current.device() && tokens->dim() == 2 &&
+                    tokens->size(0) == rows && tokens->is_contiguous() &&
+                    (tokens->scalar_type() == at::kLong || tokens->scalar_type() == at::kInt),
+                op, ": tokens must be contiguous int32 or int64 [", rows, ", history], got ",
+                tokens->sizes());
+    check_vector(*lens, rows, at::kInt, current, op, "lens");
+  }
+  c10::DeviceGuard guard(current.device());
+  const int64_t capacity = some ? tokens->size(1) : 0;
+  TVR_TRY(tvr_advance_tokens(
+      static_cast<int64_t*>(current.data_ptr()), static_cast<const int64_t*>(next.data_ptr()),
+      static_cast<const int64_t*>(slots.data_ptr()), some ? tokens->data_ptr() : nullptr,
+      some && tokens->scalar_type() == at::kLong ? 64 : 32, capacity,
+      some ? static_cast<int32_t*>(lens->data_ptr()) : nullptr, rows, capacity,
+      current_stream_handle()));
+}
+
 }  // namespace
 }  // namespace tvarant::ops
 
@@ -329,6 +359,8 @@ TORCH_LIBRARY_FRAGMENT(tvarant, m) {
         "Tensor? frequency=None, Tensor? bias_ids=None, Tensor? bias_values=None, "
         "Tensor? bias_counts=None, Tensor? masks=None, Tensor? mask_rows=None) -> Tensor");
   m.def("history_append_(Tensor(a!) tokens, Tensor(b!) lens, Tensor ids, Tensor? live=None) -> ()");
+  m.def("advance_tokens_(Tensor(a!) current, Tensor next, Tensor slots, Tensor(b!)? tokens=None, "
+        "Tensor(c!)? lens=None) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(tvarant, PrivateUse1, m) {
@@ -338,4 +370,5 @@ TORCH_LIBRARY_IMPL(tvarant, PrivateUse1, m) {
   m.impl("paged_attention_append", TORCH_FN(tvarant::ops::paged_attention_append));
   m.impl("adjust_logits", TORCH_FN(tvarant::ops::adjust_logits));
   m.impl("history_append_", TORCH_FN(tvarant::ops::history_append_));
+  m.impl("advance_tokens_", TORCH_FN(tvarant::ops::advance_tokens_));
 }

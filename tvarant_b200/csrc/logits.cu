@@ -1,7 +1,8 @@
 // Logits of a decode step adjusted before the next token is chosen
 // (tvr_adjust_logits): penalties for tokens of the history, sparse biases,
-// grammar masks; and the histories' growth by the chosen tokens
-// (tvr_history_append).
+// grammar masks; the histories' growth by the chosen tokens
+// (tvr_history_append), and their taking the place of the current ones
+// (tvr_advance_tokens).
 #include "tc_ptx.cuh"
 
 #include <algorithm>
@@ -348,16 +349,46 @@ __global__ void __launch_bounds__(kThreads)
   if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
+// A thread a row.  Rows count where live[row] > 0 or, with `slots`, where
+// slots[row] >= 0; `current` (null: none) takes ids[row] as well.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     history_append_kernel(T* tokens, int64_t stride, int32_t* lens, const int64_t* ids,
-                          const int32_t* live, int64_t rows, int64_t capacity) {
+                          const int32_t* live, const int64_t* slots, int64_t* current, int64_t rows,
+                          int64_t capacity) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (row >= rows || (live != nullptr && live[row] <= 0)) return;
+  if (slots != nullptr && slots[row] < 0) return;
+  const int64_t id = ids[row];
+  if (current != nullptr) current[row] = id;
+  if (lens == nullptr) return;
   const int at = lens[row];
   if (at < 0 || at >= capacity) return;
-  tokens[row * stride + at] = static_cast<T>(ids[row]);
+  tokens[row * stride + at] = static_cast<T>(id);
   lens[row] = at + 1;
+}
+
+int append_history(const char* op, void* tokens, int token_bits, int64_t stride, int32_t* lens,
+                   const int64_t* ids, const int32_t* live, const int64_t* slots,
+                   int64_t* current, int64_t rows, int64_t capacity, void* stream) {
+  TVR_CHECK(rows >= 0 && capacity >= 0, "%s: negative size", op);
+  TVR_CHECK(token_bits == 32 || token_bits == 64, "%s: token_bits %d", op, token_bits);
+  TVR_CHECK(capacity <= 0x7fffffff && rows <= 0x7fffffff, "%s: size past 32 bits", op);
+  if (rows == 0) return TVR_OK;
+  TVR_CHECK(ids && (lens || current) && (tokens || lens == nullptr || capacity == 0),
+            "%s: null pointer", op);
+  TVR_CHECK(lens == nullptr || rows == 1 || stride >= capacity,
+            "%s: the row stride is less than the capacity", op);
+  const unsigned grid = static_cast<unsigned>(ceil_div(rows, kThreads));
+  if (token_bits == 64) {
+    history_append_kernel<int64_t><<<grid, kThreads, 0, as_stream(stream)>>>(
+        static_cast<int64_t*>(tokens), stride, lens, ids, live, slots, current, rows, capacity);
+  } else {
+    history_append_kernel<int32_t><<<grid, kThreads, 0, as_stream(stream)>>>(
+        static_cast<int32_t*>(tokens), stride, lens, ids, live, slots, current, rows, capacity);
+  }
+  TVR_LAUNCH_CHECK();
+  return TVR_OK;
 }
 
 }  // namespace
@@ -447,21 +478,14 @@ extern "C" int tvr_adjust_logits(const float* logits, int64_t logits_stride, flo
 extern "C" int tvr_history_append(void* tokens, int token_bits, int64_t tokens_stride,
                                   int32_t* lens, const int64_t* ids, const int32_t* live,
                                   int64_t rows, int64_t capacity, void* stream) {
-  TVR_CHECK(rows >= 0 && capacity >= 0, "history_append: negative size");
-  TVR_CHECK(token_bits == 32 || token_bits == 64, "history_append: token_bits %d", token_bits);
-  TVR_CHECK(capacity <= 0x7fffffff && rows <= 0x7fffffff, "history_append: size past 32 bits");
-  if (rows == 0) return TVR_OK;
-  TVR_CHECK(lens && ids && (tokens || capacity == 0), "history_append: null pointer");
-  TVR_CHECK(rows == 1 || tokens_stride >= capacity,
-            "history_append: the row stride is less than the capacity");
-  const unsigned grid = static_cast<unsigned>(ceil_div(rows, kThreads));
-  if (token_bits == 64) {
-    history_append_kernel<int64_t><<<grid, kThreads, 0, as_stream(stream)>>>(
-        static_cast<int64_t*>(tokens), tokens_stride, lens, ids, live, rows, capacity);
-  } else {
-    history_append_kernel<int32_t><<<grid, kThreads, 0, as_stream(stream)>>>(
-        static_cast<int32_t*>(tokens), tokens_stride, lens, ids, live, rows, capacity);
-  }
-  TVR_LAUNCH_CHECK();
-  return TVR_OK;
+  return append_history("history_append", tokens, token_bits, tokens_stride, lens, ids, live,
+                        nullptr, nullptr, rows, capacity, stream);
+}
+
+extern "C" int tvr_advance_tokens(int64_t* current, const int64_t* next, const int64_t* slots,
+                                  void* tokens, int token_bits, int64_t tokens_stride,
+                                  int32_t* lens, int64_t rows, int64_t capacity, void* stream) {
+  TVR_CHECK(rows <= 0 || (current && slots), "advance_tokens: null pointer");
+  return append_history("advance_tokens", tokens, token_bits, tokens_stride, lens, next, nullptr,
+                        slots, current, rows, capacity, stream);
 }

@@ -337,8 +337,10 @@ def paged_decode_step(model: GPT2, ids: torch.Tensor, cache: PagedCache, live: t
     current tokens; each live request's is appended to its own pages and
     attends to all of its positions.  ``rules`` adjust the logits before the
     choice, and their histories take the chosen tokens.  Writes the next
-    tokens into ``ids`` and returns it (rows that are not live hold no token).
-    Nothing depends on host values, so the step can be captured once as a CUDA
+    tokens into ``ids`` and returns it.  A request that does not advance (it is
+    not live, or the pool has no page for it, which the device status word
+    says) keeps its token in ``ids``, its history and its length: a later step
+    goes on from there.  Nothing depends on host values, so the step can be captured once as a CUDA
     graph (``tvarant_b200.graphs.Graph``) and replayed while requests come and
     go."""
     F = torch.nn.functional
@@ -359,10 +361,11 @@ def paged_decode_step(model: GPT2, ids: torch.Tensor, cache: PagedCache, live: t
     logits = head(model, x).view(R, cfg.vocab)
     if rules is not None:
         logits = rules.apply(logits)
-    nxt = logits.argmax(-1)
-    if rules is not None and rules.tokens is not None:
-        torch.ops.tvarant.history_append_(rules.tokens, rules.total_lens, nxt, live)
-    ids.copy_(nxt.view(R, 1))
+    histories = () if rules is None or rules.tokens is None else (rules.tokens, rules.total_lens)
+    current = ids.long().contiguous()  # ids itself, unless it is strided or int32
+    torch.ops.tvarant.advance_tokens_(current, logits.argmax(-1), slots, *histories)
+    if current.data_ptr() != ids.data_ptr():
+        ids.copy_(current)
     return ids
 
 
