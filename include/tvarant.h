@@ -340,6 +340,7 @@ typedef struct tvr_page_pool {
   int32_t* free_pages;
   int64_t num_pages;
   int64_t page_size;
+  int64_t max_positions; /* of a request; 0: max_pages * page_size */
 } tvr_page_pool;
 
 /* One step's block tables and slot maps from request lengths, all of it on
@@ -351,8 +352,8 @@ typedef struct tvr_page_pool {
  *     pages.  In the order of the requests, pages are taken from the top of
  *     the stack and appended to the request's table row.  The first request
  *     that needs more pages than are left is refused, and so is every later
- *     one that needs a page; so is one that would exceed max_pages or whose
- *     tokens exceed the token arrays.  A refused request keeps its length and
+ *     one that needs a page; so is one that would exceed max_pages or
+ *     max_positions, or whose tokens exceed the token arrays.  A refused request keeps its length and
  *     its table, and TVR_DEV_CACHE_FULL is set in the device status word.
  *   - The tokens lie packed in the order of the requests (tokens_per_request
  *     0: request r's token i at index i + sum of the earlier requests' new

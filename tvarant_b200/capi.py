@@ -79,6 +79,7 @@ class PagePool(ctypes.Structure):
         ("free_pages", ctypes.c_void_p),
         ("num_pages", ctypes.c_int64),
         ("page_size", ctypes.c_int64),
+        ("max_positions", ctypes.c_int64),
     ]
 
 

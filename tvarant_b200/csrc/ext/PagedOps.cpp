@@ -69,14 +69,16 @@ at::Tensor unit_last(const at::Tensor& t) {
 // block_table [R, max pages] int32 and free_pages [pages] int32 are updated
 // in place, seq_lens [R] and free_count [1] too; returns slots (int64),
 // positions and rows (int32) of the step's tokens: packed [tokens], or
-// [R, tokens_per_request] where that is given (tokens is then ignored).
+// [R, tokens_per_request] where that is given (tokens is then ignored).  A
+// request has max_len positions at most (0: what its table row holds).
 std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(at::Tensor& block_table,
                                                          at::Tensor& seq_lens,
                                                          const at::Tensor& new_lens,
                                                          at::Tensor& free_pages,
                                                          at::Tensor& free_count, int64_t page_size,
                                                          int64_t tokens,
-                                                         int64_t tokens_per_request) {
+                                                         int64_t tokens_per_request,
+                                                         int64_t max_len) {
   constexpr const char* op = "page_plan";
   TORCH_CHECK(is_device(block_table) && block_table.scalar_type() == at::kInt &&
                   block_table.dim() == 2 &&
@@ -104,6 +106,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> page_plan(at::Tensor& block_table
   pool.free_pages = static_cast<int32_t*>(free_pages.data_ptr());
   pool.num_pages = free_pages.numel();
   pool.page_size = page_size;
+  pool.max_positions = max_len;
   auto ints = [](const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
   TVR_TRY(tvr_page_plan(&pool, ints(seq_lens), ints(new_lens), ints(seq_lens), ints(free_count),
                         ints(free_count), static_cast<int64_t*>(slots.data_ptr()),
@@ -344,7 +347,7 @@ void advance_tokens_(at::Tensor& current, const at::Tensor& next, const at::Tens
 TORCH_LIBRARY_FRAGMENT(tvarant, m) {
   m.def("page_plan(Tensor(a!) block_table, Tensor(b!) seq_lens, Tensor new_lens, "
         "Tensor(c!) free_pages, Tensor(d!) free_count, int page_size, int tokens, "
-        "int tokens_per_request=0) -> (Tensor, Tensor, Tensor)");
+        "int tokens_per_request=0, int max_len=0) -> (Tensor, Tensor, Tensor)");
   m.def("paged_append_(Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor k_new, Tensor v_new, "
         "Tensor slots) -> ()");
   m.def("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor block_table, "

@@ -41,6 +41,7 @@ struct PlanParams {
   int32_t* table;
   int64_t table_stride;
   int max_pages;
+  int most;  // positions of a request
   int requests;
   int32_t* free_pages;
   int num_pages;
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(const __grid_constan
     } else {
       const int want = pages_of(static_cast<long long>(seq) + grow);
       const bool room = p.per_request == 0 || grow <= p.per_request;
-      own.need = room && want <= p.max_pages ? want - held : 0;
+      own.need = room && static_cast<long long>(seq) + grow <= p.most ? want - held : 0;
       own.tokens = grow;
       held_seq = seq;
     }
@@ -167,15 +168,15 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(const __grid_constan
   }
   __syncthreads();
   const int top = free_count + before.released;
-  // Admitted: a request that fits its table row and the token arrays, and
+  // Admitted: a request that fits its positions and the token arrays, and
   // needs no page or ends within the stack.  The sums count every request that
-  // fits its row, so the first one past the stack refuses all that need a page
+  // fits its positions, so the first one past the stack refuses all that need a page
   // after it, and the first one past packed token arrays all that bring tokens.
   auto admitted = [&](int r) -> bool {
     const int seq = s_seq[r];
     if (seq < 0) return false;
     const long long first = r > 0 ? s_tokens[r - 1] : 0, grow = s_tokens[r] - first;
-    if (pages_of(seq + grow) > p.max_pages) return false;
+    if (seq + grow > p.most) return false;
     if (p.per_request > 0 ? grow > p.per_request : grow > 0 && s_tokens[r] > p.tokens) return false;
     const int need = s_need[r] - (r > 0 ? s_need[r - 1] : 0);
     return need == 0 || s_need[r] <= top;
@@ -405,7 +406,7 @@ extern "C" int tvr_page_plan(const tvr_page_pool* pool, const int32_t* seq_lens,
   using namespace paged;
   TVR_CHECK(pool != nullptr, "page_plan: null pool");
   TVR_CHECK(pool->requests >= 0 && pool->max_pages >= 0 && pool->num_pages >= 0 && tokens >= 0 &&
-                tokens_per_request >= 0,
+                tokens_per_request >= 0 && pool->max_positions >= 0,
             "page_plan: negative size");
   TVR_CHECK(pool->page_size >= 1 && pool->page_size <= (1 << 20),
             "page_plan: page size %lld is not in 1..2^20", (long long)pool->page_size);
@@ -432,6 +433,8 @@ extern "C" int tvr_page_plan(const tvr_page_pool* pool, const int32_t* seq_lens,
   p.table = pool->block_table;
   p.table_stride = pool->table_stride;
   p.max_pages = static_cast<int>(pool->max_pages);
+  p.most = static_cast<int>(pool->max_pages * pool->page_size);
+  if (pool->max_positions > 0) p.most = static_cast<int>(std::min<int64_t>(p.most, pool->max_positions));
   p.requests = static_cast<int>(pool->requests);
   p.free_pages = pool->free_pages;
   p.num_pages = static_cast<int>(pool->num_pages);

@@ -297,10 +297,25 @@ def decode_step(model: GPT2, ids: torch.Tensor, cache: KVCache, pos: torch.Tenso
 
 def new_paged_cache(model: GPT2, requests: int, num_pages: int, page_size: int, max_len: int,
                     device, dtype: torch.dtype = torch.float32) -> PagedCache:
-    """A paged cache of the model's layers and heads (``tvarant_b200.paged``)."""
+    """A paged cache of the model's layers and heads (``tvarant_b200.paged``),
+    for requests of up to ``max_len`` positions, ``n_ctx`` at most."""
     cfg = model.cfg
+    if max_len > cfg.n_ctx:
+        raise ValueError(f"{max_len} positions exceed the model's context of {cfg.n_ctx}")
     return paged.new_paged_cache(cfg.n_layer, requests, num_pages, page_size, max_len, cfg.n_head,
                                  cfg.n_head, cfg.d_model // cfg.n_head, device, dtype)
+
+
+def _check_positions(model: GPT2, cache: PagedCache, tokens: int = 0) -> None:
+    """Refuses a cache that could grow past the model's positions (an embedding
+    past its table is zero on the tvarant device), and more tokens than a
+    request of it can have."""
+    most = cache.max_positions
+    if most > model.cfg.n_ctx:
+        raise ValueError(f"a cache for requests of {most} positions exceeds the model's context "
+                         f"of {model.cfg.n_ctx}")
+    if tokens > most:
+        raise ValueError(f"{tokens} positions exceed the cache's {most}")
 
 
 def paged_prefill(model: GPT2, ids: torch.Tensor, cache: PagedCache, request: int) -> torch.Tensor:
@@ -311,6 +326,7 @@ def paged_prefill(model: GPT2, ids: torch.Tensor, cache: PagedCache, request: in
     F = torch.nn.functional
     cfg = model.cfg
     S, d, H = ids.shape[1], cfg.d_model, cfg.n_head
+    _check_positions(model, cache, S)
     hd = d // H
     scale = 1.0 / math.sqrt(hd)
     new_lens = torch.zeros(cache.requests, dtype=torch.int32)
@@ -338,14 +354,16 @@ def paged_decode_step(model: GPT2, ids: torch.Tensor, cache: PagedCache, live: t
     attends to all of its positions.  ``rules`` adjust the logits before the
     choice, and their histories take the chosen tokens.  Writes the next
     tokens into ``ids`` and returns it.  A request that does not advance (it is
-    not live, or the pool has no page for it, which the device status word
-    says) keeps its token in ``ids``, its history and its length: a later step
-    goes on from there.  Nothing depends on host values, so the step can be captured once as a CUDA
+    not live, the pool has no page for it, or it has the cache's ``max_len``
+    positions; the device status word says of the last two) keeps its token in
+    ``ids``, its history and its length: a later step goes on from there.
+    Nothing depends on host values, so the step can be captured once as a CUDA
     graph (``tvarant_b200.graphs.Graph``) and replayed while requests come and
     go."""
     F = torch.nn.functional
     cfg = model.cfg
     R, d, H = ids.shape[0], cfg.d_model, cfg.n_head
+    _check_positions(model, cache)
     hd = d // H
     scale = 1.0 / math.sqrt(hd)
     slots, positions, _ = cache.plan(live, tokens_per_request=1)

@@ -24,7 +24,8 @@ class PagedCache:
     float32, float16 or bfloat16 (new rows are rounded to it; attention
     computes in fp32).  ``block_table`` ``[requests, max pages]``, ``seq_lens``
     ``[requests]``, ``free_pages`` and ``free_count`` are int32.
-    ``workspace`` belongs to the attention calls: two steps that may run at
+    A request has at most ``max_len`` positions (0: what its row of the table
+    holds).  ``workspace`` belongs to the attention calls: two steps that may run at
     the same time need a cache object with a workspace of its own each.
     """
 
@@ -35,6 +36,7 @@ class PagedCache:
     free_pages: torch.Tensor
     free_count: torch.Tensor
     workspace: torch.Tensor
+    max_len: int = 0
 
     @property
     def requests(self) -> int:
@@ -44,17 +46,23 @@ class PagedCache:
     def page_size(self) -> int:
         return self.k[0].shape[2]
 
+    @property
+    def max_positions(self) -> int:
+        """The positions that a request can have."""
+        held = self.block_table.shape[1] * self.page_size
+        return min(held, self.max_len) if self.max_len > 0 else held
+
     def plan(self, new_lens: torch.Tensor, tokens: int = 0, tokens_per_request: int = 0):
         """Block tables and slot maps for ``new_lens[r]`` new tokens of each
         request (int32, on the device; negative: the request ends and gives up
         its pages).  Returns ``(slots, positions, rows)`` of the tokens, packed
         ``[tokens]`` in the order of the requests, or ``[requests,
-        tokens_per_request]``.  A request that the pool cannot serve keeps its
-        length, its slots are -1, and the device status word becomes 7
+        tokens_per_request]``.  A request that the pool cannot serve, or that
+        would have more than ``max_positions``, keeps its length, its slots are -1, and the device status word becomes 7
         (``TVR_DEV_CACHE_FULL``)."""
         return torch.ops.tvarant.page_plan(self.block_table, self.seq_lens, new_lens,
                                            self.free_pages, self.free_count, self.page_size,
-                                           tokens, tokens_per_request)
+                                           tokens, tokens_per_request, self.max_len)
 
     def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor,
                slots: torch.Tensor) -> None:
@@ -99,7 +107,7 @@ def new_paged_cache(layers: int, requests: int, num_pages: int, page_size: int, 
                       ints(torch.zeros(requests)),
                       ints(torch.arange(num_pages - 1, -1, -1)),  # page 0 on top
                       ints(torch.tensor([num_pages])),
-                      torch.zeros(max(1, size), dtype=torch.uint8, device=device))
+                      torch.zeros(max(1, size), dtype=torch.uint8, device=device), max_len)
 
 
 @dataclass
