@@ -384,8 +384,9 @@ int tvr_paged_append(const tvr_paged_kv* cache, const float* k_new, const float*
  *   out[r, h] = softmax_j(scale q[r, h] . k[r, g, j]) v[r, g, j],
  *   g = h / (heads / kv_heads), j < seq_lens[r],
  * and lse[r, h] (NULL: not wanted), the natural-log log-sum-exp.  A request
- * of length 0 (or less) gives a zero row and lse = -inf; a length past the
- * table counts as max_pages * page_size.  Products and sums are fp32 whatever
+ * of length 0 (or less), or none of whose positions counts (below), gives a
+ * zero row and lse = -inf; a length past the table counts as max_pages *
+ * page_size.  Products and sums are fp32 whatever
  * the pages' type.  q and out are [requests, heads, head_dim], k_new and
  * v_new [requests, kv_heads, head_dim], fp32; strides holds the (request,
  * head) element strides of q, k_new, v_new and out, in that order.

@@ -47,7 +47,9 @@ struct AttendParams {
 // to the warps in turn; each warp keeps a running maximum and sum (exp2
 // domain) and the CTA joins the warps at the end.  The maximum starts at
 // -FLT_MAX, not -inf, so that a score of -inf gives a weight of 0 without a
-// special case and a row of nothing but -inf gives 0 / 0, as the formula does.
+// special case and a row of nothing but -inf gives 0 / 0, as the formula does;
+// a row without any position that counts (length 0, or all of its page ids out
+// of range) is told apart from it and gives zeros.
 // Bound by latency, a key at a time (128 requests of 200 to 8000 keys, 12 heads
 // of 64, fp32 pages: 1708 us; the streaming form below 257 us), so it takes only
 // what the other cannot: rows that are not whole 16-byte chunks.
@@ -76,6 +78,7 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
     o[i] = 0.f;
   }
   float m = -FLT_MAX, l = 0.f;
+  bool counted = false;  // whether any position of this warp counts
   for (int j = warp; j < n; j += kGeneralWarps) {
     float k[DL], v[DL];
     if (fresh && j == n - 1) {
@@ -117,6 +120,7 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
         v[i] = d < p.dim ? to_f32(vc[d]) : 0.f;
       }
     }
+    counted = true;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < DL; ++i) s = fmaf(q[i], k[i], s);
@@ -135,17 +139,17 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
   }
 #pragma unroll
   for (int i = 0; i < DL; ++i) s_o[warp][lane + 32 * i] = o[i];
-  __syncthreads();
+  const bool some = __syncthreads_or(counted) != 0;
   float top = -FLT_MAX, sum = 0.f;
   for (int w = 0; w < kGeneralWarps; ++w) top = fmaxf(top, s_m[w]);
   for (int w = 0; w < kGeneralWarps; ++w) sum += s_l[w] * exp2f(s_m[w] - top);
   for (int d = threadIdx.x; d < p.dim; d += 32 * kGeneralWarps) {
     float acc = 0.f;
     for (int w = 0; w < kGeneralWarps; ++w) acc += s_o[w][d] * exp2f(s_m[w] - top);
-    p.out[r * p.o_s[0] + h * p.o_s[1] + d] = n > 0 ? acc / sum : 0.f;
+    p.out[r * p.o_s[0] + h * p.o_s[1] + d] = some ? acc / sum : 0.f;
   }
   if (threadIdx.x == 0 && p.lse != nullptr) {
-    p.lse[r * p.heads + h] = n > 0 ? top * 0.69314718055994531f + logf(sum) : -INFINITY;
+    p.lse[r * p.heads + h] = some ? top * 0.69314718055994531f + logf(sum) : -INFINITY;
   }
 }
 
@@ -264,7 +268,8 @@ struct Stream {
   static constexpr int kSmem = dynamic_bytes(kStages);
   static_assert(kStages >= 2 && kKeys <= 16, "the ring");
   static_assert(MT == 0 || kStage >= kHeads * (DP + 8) * 4, "a part takes the place of a stage");
-  static constexpr int kRecord = DP + 4;  // floats of one head's part: output, maximum, sum
+  // floats of one head's part: output, maximum, sum, whether a position counts
+  static constexpr int kRecord = DP + 4;
 };
 
 struct StreamParams {
@@ -710,6 +715,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     }
     const int h0 = g * p.group + sub * HEADS;
     const int heads = min(HEADS, p.group - sub * HEADS);
+    bool counted = false;  // whether any position of this warp's counts
     // the segment after this one begins a unit, if there is one
     const bool follow = u + (t1 - t0) < u_end;
     const int n_unit = unit + 1 < units ? unit + 1 : 0, n_request = r + (unit + 1 < units ? 0 : 1);
@@ -752,6 +758,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
         ready();
         const uint32_t kd = ring + get * S::kStage, vd = kd + S::kHalf;
         const uint32_t live = s_live[warp][get];
+        counted |= live != 0;
 #pragma unroll
         for (int it = 0; it < KEYS / STEP; ++it) {
           const int row = it * STEP + lane / L;
@@ -919,6 +926,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
         ready();
         const uint32_t kd = ring + get * S::kStage, vd = kd + S::kHalf;
         const uint32_t live = s_live[warp][get];
+        counted |= live != 0;
 
         // ---- scores
         constexpr int CHAINS = sizeof(T) == 4 ? 2 : 1;
@@ -1170,7 +1178,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     // ---- on to the next segment, whose copies are under way while the parts
     // of this one are joined
     const int d_r = r, d_count = count;
-    const bool whole = real0 == 0 && t1 == count, empty = n == 0;
+    const bool whole = real0 == 0 && t1 == count;
     const int real_from = real0;
     const long long u_unit = u - t0;  // the unit's first tile
     constexpr int kPartStep = MT == 0 ? DP : S::kWarpRing / 4;  // floats between warps' parts
@@ -1196,7 +1204,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
     }
 
     // ---- the warps' parts into one
-    __syncthreads();
+    const bool empty = __syncthreads_or(counted) == 0;
     if (tid < HEADS) {
       float top = -FLT_MAX, sum = 0.f;
 #pragma unroll
@@ -1239,6 +1247,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
       if (!whole) {
         part[tid * S::kRecord + DP] = s_top[tid];
         part[tid * S::kRecord + DP + 1] = s_sum[tid];
+        part[tid * S::kRecord + DP + 2] = empty ? 0.f : 1.f;
       } else if (lse != nullptr) {
         lse[tid] = empty ? -INFINITY : s_top[tid] * 0.69314718055994531f + logf(s_sum[tid]);
       }
@@ -1275,13 +1284,14 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
           sum = sum * exp2f(top - to) + l * exp2f(m - to);
           top = to;
         };
-        float top = -FLT_MAX, sum = 0.f;
+        float top = -FLT_MAX, sum = 0.f, some = 0.f;
         if (tid % HEADS < heads) {
 #pragma unroll 4
           for (int x = tid; x < count * HEADS; x += THREADS) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(
+            const float4 mls = __ldcg(reinterpret_cast<const float4*>(
                 record(from + x / HEADS * every) + x % HEADS * S::kRecord + DP));
-            merge(top, sum, ml.x, ml.y);
+            merge(top, sum, mls.x, mls.y);
+            some = fmaxf(some, mls.z);
           }
         }
 #pragma unroll
@@ -1293,7 +1303,7 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
           s_m[warp][lane] = top;
           s_l[warp][lane] = sum;
         }
-        __syncthreads();
+        const bool none = __syncthreads_or(some != 0.f) == 0;
         if (tid < heads) {
           top = s_m[0][tid];
           sum = s_l[0][tid];
@@ -1301,8 +1311,10 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
           for (int w = 1; w < WARPS; ++w) merge(top, sum, s_m[w][tid], s_l[w][tid]);
           s_top[tid] = top;
           s_sum[tid] = sum;
-          s_inverse[tid] = 1.f / sum;
-          if (into_outputs && lse != nullptr) lse[tid] = top * 0.69314718055994531f + logf(sum);
+          s_inverse[tid] = none ? 0.f : 1.f / sum;
+          if (into_outputs && lse != nullptr) {
+            lse[tid] = none ? -INFINITY : top * 0.69314718055994531f + logf(sum);
+          }
         }
         __syncthreads();
         // LANES lanes read a part's outputs, 16 bytes each and VECS of them;
@@ -1358,8 +1370,8 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
           }
         }
         if (!into_outputs && tid < heads) {
-          *reinterpret_cast<float2*>(into + tid * S::kRecord + DP) =
-              make_float2(s_top[tid], s_sum[tid]);
+          *reinterpret_cast<float4*>(into + tid * S::kRecord + DP) =
+              make_float4(s_top[tid], s_sum[tid], none ? 0.f : 1.f, 0.f);
         }
       };
       if (n_parts <= kJoinAtOnce) {
