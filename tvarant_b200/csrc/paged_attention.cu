@@ -1004,7 +1004,10 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
               if constexpr (PACKED) v += __shfl_xor_sync(FULL, v, 16);
               const bool in = ((live >> (nt * 8 + 2 * thr + e)) & 1u) != 0;
               z[mt][nt][e] = in ? v : -INFINITY;
-              over |= z[mt][nt][e] > m[mt] + (LIFT + kSlack);
+              // of the difference, which is what the weight is made of: past
+              // 2^25, m + 15 may round up to m + 16, and an f16 weight of 2^16
+              // is an infinity
+              over |= z[mt][nt][e] - m[mt] > LIFT + kSlack;
             }
           }
         }
