@@ -1,5 +1,5 @@
-"""Scores so large that their rounding shows: the outputs stay finite, and equal
-to the formula where the scores' bits decide it."""
+"""Scores and queries so large that their rounding or their range shows: the
+outputs stay finite, and equal to the formula where the scores' bits decide it."""
 
 from __future__ import annotations
 
@@ -64,3 +64,22 @@ def test_outputs_stay_finite(lib, heads, kv_heads, dim, dtype):  # noqa: F811
         for step in (2.0, 8.0, 16.0, 64.0):
             out, lse = _two_levels(lib, heads, kv_heads, dim, dtype, power, step).run()
             assert np.isfinite(out).all() and np.isfinite(lse).all(), (power, step)
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, dtype", F16 + OTHERS)
+def test_queries_near_the_largest(lib, heads, kv_heads, dim, dtype):  # noqa: F811
+    """Queries of 2^118: the position of the largest score takes all of the
+    weight, and its value is the output, to the 22 bits of an fp32 value's two
+    terms at least."""
+    c = Case(lib, [50, 200], heads, kv_heads, dim, 16, dtype)
+    c.q *= 2.0**118
+    out, _ = c.run()
+    q = c.q.cpu().double().numpy()
+    for r in range(2):
+        k, v = c.rows[r]
+        for h in range(heads):
+            g = h // (heads // kv_heads)
+            z = np.sort(k[g] @ q[r, h])
+            if z[-1] - z[-2] > 1e-4 * abs(z[-1]):  # not a tie within the scores' errors
+                one = v[g, np.argmax(k[g] @ q[r, h])]
+                assert np.max(np.abs(out[r, h] - one)) <= 2.0**-20 * np.max(np.abs(one))

@@ -863,9 +863,10 @@ __global__ void __launch_bounds__(Stream<T, DP, MT, PACKED>::kThreads,
           for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
 #pragma unroll
           for (int d = 1; d < DP / 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
-          // 2^(13 - exponent of top), within the range of fp32
+          // 2^(13 - exponent of top): down to 2^-114, up to 2^100 (smaller
+          // queries make scores that are zero to fp32's last bit all the same)
           const int e2 = static_cast<int>((__float_as_uint(top) >> 23) & 255u);
-          const int lift = e2 == 0 || e2 == 255 ? 0 : max(-100, min(100, 13 - (e2 - 127)));
+          const int lift = e2 == 0 || e2 == 255 ? 0 : min(100, 13 - (e2 - 127));
           const float up = __uint_as_float(static_cast<uint32_t>(127 + lift) << 23);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= up;
