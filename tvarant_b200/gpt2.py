@@ -322,7 +322,9 @@ def paged_prefill(model: GPT2, ids: torch.Tensor, cache: PagedCache, request: in
     """Takes the prompt ``ids`` [1, S] (int64, device) of a fresh request into
     the cache and returns its logits [1, S, vocab], those of ``forward``.  The
     other requests are as they were.  The pool must have the pages (the device
-    status word says if it had not)."""
+    status word says if it had not).  The caller chooses the first token after
+    the prompt; where the choices have rules, ``LogitRules.row`` applies them
+    to it and takes it into the history."""
     F = torch.nn.functional
     cfg = model.cfg
     S, d, H = ids.shape[1], cfg.d_model, cfg.n_head

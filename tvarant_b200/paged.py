@@ -115,7 +115,8 @@ class LogitRules:
     """What ``torch.ops.tvarant.adjust_logits`` applies to the logits of a step
     (include/tvarant.h, ``tvr_adjust_logits``); an absent part is None.  With
     ``tokens`` the histories grow by the tokens that
-    ``gpt2.paged_decode_step`` chooses."""
+    ``gpt2.paged_decode_step`` chooses.  A prompt's tokens, and the first token
+    after it (``row``), are for the caller to put there."""
 
     tokens: torch.Tensor | None = None        # [requests, capacity] int32 or int64
     prompt_lens: torch.Tensor | None = None   # [requests] int32
@@ -128,6 +129,24 @@ class LogitRules:
     bias_counts: torch.Tensor | None = None   # [requests] int32
     masks: torch.Tensor | None = None         # [masks, words] int32, a bit a token
     mask_rows: torch.Tensor | None = None     # [requests] int32, -1: no mask
+
+    def row(self, r: int) -> LogitRules:
+        """The rules of request ``r`` alone, for logits ``[1, vocab]``: views, so
+        that its history grows in place.  The first token after a prompt, with
+        ``logits`` from ``gpt2.paged_prefill``::
+
+            one = rules.row(r)
+            first = one.apply(logits[:, -1]).argmax(-1)
+            torch.ops.tvarant.history_append_(one.tokens, one.total_lens, first)
+        """
+        def cut(t):
+            return None if t is None else t[r:r + 1]
+
+        return LogitRules(
+            cut(self.tokens), cut(self.prompt_lens), cut(self.total_lens), cut(self.repetition),
+            cut(self.presence), cut(self.frequency), cut(self.bias_ids), cut(self.bias_values),
+            cut(self.bias_counts), self.masks if self.mask_rows is not None else cut(self.masks),
+            cut(self.mask_rows))
 
     def apply(self, logits: torch.Tensor) -> torch.Tensor:
         return torch.ops.tvarant.adjust_logits(
