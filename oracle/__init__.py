@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import unittest
 from pathlib import Path
 
 import numpy as np
@@ -49,17 +50,22 @@ def available(impl: str = "port") -> bool:
     return (PORT_LIB if impl == "port" else REF_LIB).exists()
 
 
+class ReferenceAbsent(FileNotFoundError, unittest.SkipTest):
+    """The reference's library is not built and its sources are not there to
+    build it from: what compares with it is skipped."""
+
+
 def _lib(impl: str) -> ctypes.CDLL:
     if impl in _libs:
         return _libs[impl]
     path = PORT_LIB if impl == "port" else REF_LIB
     if not path.exists():
-        if impl == "port":
-            from . import build as _build
+        from . import build as _build
 
+        if impl == "port":
             _build.build_oracle()
-        else:
-            raise FileNotFoundError(f"{path} not built (python oracle/build.py)")
+        elif _build.build_reference() is None:
+            raise ReferenceAbsent(f"{path} not built: the reference's sources are not present")
     lib = ctypes.CDLL(str(path))
     pre = "tvo_" if impl == "port" else "ref_"
     vp = ctypes.c_void_p
