@@ -386,16 +386,24 @@ int tvr_paged_append(const tvr_paged_kv* cache, const float* k_new, const float*
  * and lse[r, h] (NULL: not wanted), the natural-log log-sum-exp.  A request
  * of length 0 (or less), or none of whose positions counts (below), gives a
  * zero row and lse = -inf; a length past the table counts as max_pages *
- * page_size.  Products and sums are fp32 whatever
- * the pages' type.  q and out are [requests, heads, head_dim], k_new and
- * v_new [requests, kv_heads, head_dim], fp32; strides holds the (request,
- * head) element strides of q, k_new, v_new and out, in that order.
+ * page_size.  Sums are fp32 whatever the pages' type.  Products are fp32 with
+ * one head a key head; heads that share one are multiplied on the tensor
+ * cores, for which queries and weights (and the keys and values of fp32 pages)
+ * are cut into terms that together carry at least 22 of their 24 bits, and a
+ * score is summed there, where sums are cut off and not rounded: with N(0, 1)
+ * operands the outputs' relative errors are up to 2.1e-7 in the first case and
+ * 1.1e-6 in the second (fp32 pages, 256 dimensions).  q and out are [requests,
+ * heads, head_dim], k_new and v_new [requests, kv_heads, head_dim], fp32;
+ * strides holds the (request, head) element strides of q, k_new, v_new and
+ * out, in that order.
  * With k_new, v_new and slots (all three or none) the call also appends: for
  * slots[r] >= 0, position seq_lens[r] - 1 is taken from k_new / v_new (rounded
  * to the pages' type) and written to slots[r], which has to be that
  * position's slot: the same as tvr_paged_append and then this call.
- * A page id or slot out of range is dropped (the position does not count)
- * and sets TVR_DEV_BAD_INDEX.  What pages hold at positions that do not
+ * A page id out of range is dropped, its positions do not count, and sets
+ * TVR_DEV_BAD_INDEX.  So does a slot past the pages: nothing is appended, and
+ * the position counts with what the pages hold there, as after
+ * tvr_paged_append with that slot.  What pages hold at positions that do not
  * count is not used.  Keys and values at positions that count are finite: an
  * infinite or NaN one may make its request's outputs NaN where the formula
  * has a value, and reaches no other request.  head_dim is at most 256

@@ -197,7 +197,9 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
 // MT > 0, 8 MT query heads a key head: tensor cores (mma.sync with 16 rows,
 // fp32 sums), which take operands of 8 or 11 bits.  A query or weight is
 // therefore cut into terms that together carry 22 to 24 bits, each product of
-// a term with a page element is exact, and only the terms' sums are rounded:
+// a term with a page element is exact, and only the terms' sums lose bits (the
+// tensor core cuts them off: relative errors of outputs to 1.1e-6, for 1.5e-7
+// to 2.1e-7 of MT = 0):
 //   f16 pages:  x = hi + lo in f16, rows h and h + 8 of the 16.  f16 has little
 //     range, so a head's query is scaled by a power of two to 2^13 and weights
 //     by 2^7 (both are taken back exactly);
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(32 * kGeneralWarps)
 //     at most four heads (PACKED) in rows h + 4 of the same one, for which a
 //     head's scores are made in two lanes, 16 apart;
 //   f32 pages:  x = hi + lo in tf32, and so are keys and values, their hi and
-//     lo in a product each.
+//     lo in a product each; of lo's 12 or 13 bits tf32 takes 11.
 // A lane's scores are its own weights of the second product, and rows h and
 // h + 8 of a sum are in one lane: nothing is exchanged between lanes.
 constexpr int kMaxCtas = 640;  // bound on a launch's CTAs; sizes the workspace
@@ -1412,7 +1414,10 @@ struct StreamPlan {
 // where most units are cut into parts, units of 8: a part costs by its heads, and
 // the second unit's reads come from L2.  Equal at 64 (request, key head) pairs:
 // 16 heads of 128 a key head, f16, 1000 to 8000 keys, 16 pairs 34.5 us with 16
-// and 26.5 us with 8, 64 pairs 41 and 41 us, 128 pairs 61 and 74 us.
+// and 26.5 us with 8, 64 pairs 41 and 41 us, 128 pairs 61 and 74 us.  The lengths
+// are not known here; short requests are cut less and lose by it: 80 pairs of 100
+// to 1000 keys, fp32, 26.7 us with 16 and 24.9 us with 8 (64 dimensions 19.7 and
+// 17.0), f16 of 64 dimensions 13.2 and 12.5.
 constexpr int64_t kWidePairs = 64;
 
 StreamPlan stream_plan(int page_type, int64_t pairs, int64_t group, int64_t dim) {
